@@ -73,7 +73,7 @@ int muse_moe_workspace_offsets(int tokens, int top_k, int local_count, int hidde
  * failure (then a call returned garbage): 1-4 a wait of the expert GEMM's producer / MMA /
  * epilogue / dequantiser role expired, 5 the single launch's combine waited in vain for its
  * rows, 6 an expert-parallel exchange waited in vain for a peer, 7 an exchange found the
- * device's generation parity different from the caller's. Synchronous: copies from the device
+ * device's generation parity different from the caller's, 8 a wait of a dense product expired. Synchronous: copies from the device
  * on the current device; reset != 0 clears it. Not for use inside a captured graph.
  */
 int muse_moe_device_status(int* status, int reset);
@@ -365,6 +365,55 @@ int muse_moe_forward_noalloc(const void* x, const int32_t* topk_ids, const float
                              const uint8_t* w13p, const uint8_t* w13_sfp, const float* w13_gs,
                              const uint8_t* w2p, const uint8_t* w2_sfp, const float* w2_gs,
                              const void* post_norm_w, void* out, muse_stream_t stream);
+
+/*
+ * Dense products beside the routed experts. dtype: 0 bf16, 1 fp16, the type of x, add, out and of
+ * 16-bit weights; ld* are row strides in elements. out may not overlap an input.
+ *
+ * muse_moe_linear_prepared_size / muse_moe_prepare_linear: a row-major NVFP4 matrix w u8 [rows,
+ * cols/2], w_sf e4m3 [rows, cols/16] in the experts' tile order (any rows; cols a multiple of 16;
+ * rows and columns padded to 128 with zero codes). gated: rows [0, rows/2) are gate rows, the
+ * rest the matching up rows. No counterpart in the reference, whose prepare (baseline.py:82-103)
+ * repacks routed experts only.
+ */
+int muse_moe_linear_prepared_size(int rows, int cols, int gated, size_t* code_bytes, size_t* scale_bytes);
+int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int cols, int gated,
+                            uint8_t* w_out, uint8_t* w_sf_out, muse_stream_t stream);
+
+/*
+ * out[t, n] = gs * sum_k x[t, k] * e2m1[n, k] * e4m3[n, k/16] (+ add[t, n]), or with gated
+ * out[t, i] = silu(gate) * up (+ add), [tokens, rows/2]. rows, cols, gated as at the prepare call.
+ * x: 16-byte aligned, ldx a multiple of 8. fp32 sums over weights that are exact in 16 bits, one
+ * rounding at the end. No counterpart in the reference.
+ */
+int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int rows, int cols, int gated,
+                       const uint8_t* wp, const uint8_t* w_sfp, const float* w_gs, const void* add,
+                       long long ld_add, void* out, long long ldo, muse_stream_t stream);
+
+/*
+ * The gated feed-forward block with 16-bit weights w13 [2 * inter, hidden] (gate rows, then up
+ * rows) and w2 [hidden, inter]: out = (silu(x . Wg^T) * (x . Wu^T)) . W2^T (+ add), [tokens, hidden].
+ * ab: null, or fp32 [tokens, 2 * inter] that receives the pre-activations for the backward call.
+ * hidden and inter multiples of 8; pointers 16-byte aligned, row strides multiples of 8; workspace
+ * 256-byte aligned, muse_moe_ffn_workspace_size bytes, its contents need no initialisation.
+ * No counterpart in the reference (its experts are routed ones, reference.py:93-107).
+ */
+int muse_moe_ffn_workspace_size(int tokens, int hidden, int inter, int backward, size_t* bytes);
+int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int tokens, int hidden, int inter,
+                         const void* w13, long long ld13, const void* w2, long long ld2, const void* add,
+                         long long ld_add, void* out, float* ab, void* workspace, size_t workspace_bytes,
+                         muse_stream_t stream);
+
+/*
+ * Gradients of that block from dy [tokens, hidden] and the forward call's ab: dx [tokens, hidden],
+ * dw13 [2 * inter, hidden], dw2 [hidden, inter], contiguous, each null if it is not wanted (then x,
+ * w13 may be null too if no other result needs them). tokens > 0. Every sum is taken in a fixed
+ * order: equal inputs give equal bits. Device status 8: a wait inside a product expired.
+ */
+int muse_moe_ffn_backward(const void* dy, long long ldy, const void* x, long long ldx, int dtype, int tokens,
+                          int hidden, int inter, const void* w13, long long ld13, const void* w2,
+                          long long ld2, const float* ab, void* dx, void* dw13, void* dw2, void* workspace,
+                          size_t workspace_bytes, muse_stream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -15,6 +15,7 @@ LIB_NAME = "libmusemoe.so"
 # Every symbol include/muse_moe.h declares, with (restype, argtypes).
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
 _SIZE_P = ctypes.POINTER(ctypes.c_size_t)
 SIGNATURES: dict[str, tuple] = {
     "muse_moe_version": (_I, []),
@@ -59,6 +60,13 @@ SIGNATURES: dict[str, tuple] = {
                                                       ctypes.c_longlong, _P, _P]),
     "muse_moe_forward_noalloc": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I,
                                       _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "muse_moe_linear_prepared_size": (_I, [_I, _I, _I, _SIZE_P, _SIZE_P]),
+    "muse_moe_prepare_linear": (_I, [_P, _P, _I, _I, _I, _P, _P, _P]),
+    "muse_moe_linear_w4": (_I, [_P, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P, _L, _P]),
+    "muse_moe_ffn_workspace_size": (_I, [_I, _I, _I, _I, _SIZE_P]),
+    "muse_moe_ffn_forward": (_I, [_P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _P, _P, ctypes.c_size_t, _P]),
+    "muse_moe_ffn_backward": (_I, [_P, _L, _P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _P, _P,
+                                   ctypes.c_size_t, _P]),
 }
 
 # Return codes (include/muse_moe.h).

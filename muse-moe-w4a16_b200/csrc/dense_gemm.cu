@@ -1,0 +1,616 @@
+// Dense 16-bit matrix products on the 5th-generation tensor cores (tcgen05, sm_100a), for the
+// gated feed-forward block: D[m, n] = sum_k A[m, k] B[n, k], fp32 accumulators in tensor memory.
+//
+//   forward   ab = x . W13^T (A, B along k)      epilogue h = silu(a) * b, ab kept in fp32 to train
+//             y  = h . W2^T                      epilogue + add
+//   backward  dh = dy . W2 (B along n)           epilogue da, db, h from ab
+//             dx = [da db] . W13 (B along n);  dW13 = [da db]^T x, dW2 = dy^T h (A along m, B along n)
+//
+// A CTA pair (cluster of two, cta_group::2) computes a 256 x bn tile (bn <= 256): each CTA loads
+// its own 128 rows of A and half of B's columns, one thread of the leader issues M = 256 MMAs that
+// read both halves, so an SM fetches 32 KB for 2 * 128 * 256 * 64 operations and the two operands'
+// shared-memory reads stay below the port's rate. Operands that run along m or n are fetched as
+// they lie (64-wide boxes, "MN-major" descriptors): no transposed copy is made.
+// Six ring stages of 64 k; two accumulators of 256 columns, so a tile's epilogue (eight warps)
+// overlaps the next tile's MMAs. Pairs are persistent and walk a static tile list, eight row tiles
+// to a group, so that the tiles in flight share their operands in L2. With too few tiles for the
+// pairs K is split and fp32 partials are summed, in split order, by a second kernel: results do
+// not depend on timing.
+// In the gate product the leader's half of B is gate rows and its peer's half the matching up
+// rows, so one thread holds a and b of the same element.
+// Bound by: the tensor pipe for many tokens, weight bytes for few.
+#undef MUSE_TRACE  // these kernels record no stamps
+#include "dense.cuh"
+
+#include <cudaTypedefs.h>
+
+#include "kernels.cuh"
+#include "ptx.cuh"
+
+namespace muse {
+namespace {
+
+constexpr int kBm = 128;                  // rows of A per CTA (256 per pair)
+constexpr int kBk = 64;                   // k per stage: one 128-byte swizzle row
+constexpr int kMaxBn = 256;
+constexpr int kStages = 6;
+constexpr int kABytes = kBm * kBk * 2;    // 16 KiB
+constexpr int kBBytes = kMaxBn / 2 * kBk * 2;
+constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kPatch = 32 * 32 * 4;       // one epilogue warp's 32 x 32 fp32 staging patch
+constexpr int kGroupM = 8;                // row tiles per raster group
+constexpr int kWaitFailed = 8;            // device status of an expired wait here
+
+struct Ctl {
+  uint64_t full[kStages], empty[kStages];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem;
+};
+constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kEpiWarps * kPatch + sizeof(Ctl);
+static_assert(kSmem <= 232448, "shared memory of one CTA");
+
+struct Args {
+  int m, n, inter;                    // inter: I of the gate modes (0 otherwise)
+  int bn, tiles_m, tiles_n, splits, kb_total, kb_per_split;
+  int dtype, partial;                 // partial: write fp32 sums to `partials` instead
+  uint32_t idesc;
+  uint32_t tx_bytes;                  // both CTAs' bytes per stage
+  void* out;
+  long long ldo;
+  const void* add;
+  long long ld_add;
+  float* ab;
+  void* h_out;
+  float* partials;
+  int* error_flag;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Address of the same shared-memory object in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(ptx::smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// TMA box into this CTA's shared memory, completing on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Arrive on `bar` of both CTAs once this thread's MMAs so far have completed.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          ptx::smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// Shared-memory descriptors, 128-byte swizzle. K-major: rows of 64 k, 8-row groups 1024 B apart.
+// MN-major: boxes of 64 (m or n) x 64 k, 8192 B apart (the leading offset); 8-k groups 1024 B
+// apart (the stride offset).
+template <bool kMn>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)((kMn ? 8192u : 16u) >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// Descriptor step of 16 k (in 16-byte units).
+template <bool kMn>
+constexpr uint32_t kStepDesc = kMn ? 16 * 128 / 16 : 2;
+
+struct Tile {
+  int m0, n0, kb0, kb1, split;
+};
+// Work item -> tile: splits innermost, then kGroupM row tiles per column tile.
+__device__ __forceinline__ Tile tile_of(const Args& a, int w) {
+  Tile t;
+  const int idx = w / a.splits;
+  t.split = w - idx * a.splits;
+  const int group = idx / (kGroupM * a.tiles_n);
+  const int first = group * kGroupM;
+  const int rows = min(kGroupM, a.tiles_m - first);
+  const int r = idx - group * kGroupM * a.tiles_n;
+  t.m0 = (first + r % rows) * 2 * kBm;
+  t.n0 = r / rows;                         // column tile index
+  t.kb0 = t.split * a.kb_per_split;
+  t.kb1 = min(a.kb_total, t.kb0 + a.kb_per_split);
+  return t;
+}
+
+__device__ __forceinline__ void store4(int dtype, void* base, long long ld, int row, int col, float4 v) {
+  uint2 p;
+  p.x = pack16(dtype, v.x, v.y);
+  p.y = pack16(dtype, v.z, v.w);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + (size_t)row * ld + col) = p;
+}
+__device__ __forceinline__ float4 add4(int dtype, const void* base, long long ld, int row, int col, float4 v) {
+  const uint2 p = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + (size_t)row * ld + col));
+  const float2 lo = unpack16(dtype, p.x), hi = unpack16(dtype, p.y);
+  return make_float4(v.x + lo.x, v.y + lo.y, v.z + hi.x, v.w + hi.y);
+}
+// da, db and h of four elements from dh, a, b:  s = 1 / (1 + exp(-a)),
+// da = dh * b * s * (1 + a * (1 - s)), db = dh * a * s, h = a * s * b.
+__device__ __forceinline__ void dgate1(float dh, float a, float b, float& da, float& db, float& h) {
+  const float s = 1.f / (1.f + __expf(-a));
+  const float as = a * s;
+  da = dh * b * (s + as * (1.f - s));
+  db = dh * as;
+  h = as * b;
+}
+__device__ __forceinline__ void dgate4(const Args& p, int row, int col, float4 dh, float4 a, float4 b) {
+  float4 da, db, h;
+  dgate1(dh.x, a.x, b.x, da.x, db.x, h.x);
+  dgate1(dh.y, a.y, b.y, da.y, db.y, h.y);
+  dgate1(dh.z, a.z, b.z, da.z, db.z, h.z);
+  dgate1(dh.w, a.w, b.w, da.w, db.w, h.w);
+  store4(p.dtype, p.out, p.ldo, row, col, da);
+  store4(p.dtype, p.out, p.ldo, row, p.inter + col, db);
+  store4(p.dtype, p.h_out, p.inter, row, col, h);
+}
+
+// 32 x 32 fp32 patch of one warp: thread = row writes its 32 columns, then lane l reads columns
+// 4 (l % 8) .. + 3 of row 4 i + l / 8. 16-byte pieces are swizzled by the row: no bank conflicts.
+__device__ __forceinline__ void patch_put(uint8_t* patch, int lane, const float (&v)[32]) {
+#pragma unroll
+  for (int p = 0; p < 8; ++p)
+    *reinterpret_cast<float4*>(patch + lane * 128 + ((p ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+}
+__device__ __forceinline__ float4 patch_get(const uint8_t* patch, int lane, int i) {
+  const int row = 4 * i + (lane >> 3), p = lane & 7;
+  return *reinterpret_cast<const float4*>(patch + row * 128 + ((p ^ (row & 7)) << 4));
+}
+
+template <bool kAMn, bool kBMn, int kMode>
+__global__ void __launch_bounds__(kThreads, 1)
+dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* patches = smem + kStages * kStageBytes;
+  Ctl& ctl = *reinterpret_cast<Ctl*>(patches + kEpiWarps * kPatch);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int total = a.tiles_m * a.tiles_n * a.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&ctl.full[s], 1);
+      ptx::mbar_init(&ctl.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(&ctl.acc_full[b], 1);
+      ptx::mbar_init(&ctl.acc_empty[b], 2 * kEpiWarps);
+    }
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&map_a);
+    ptx::prefetch_tensormap(&map_b);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::smem_u32(&ctl.tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = ctl.tmem;
+  chain_release();
+  chain_wait();
+
+  bool ok = true;
+  if (warp == 0) {
+    if (ptx::elect_one()) {
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int w = pair; w < total && ok; w += pairs) {
+        const Tile t = tile_of(a, w);
+        const int row = t.m0 + rank * kBm;
+        const int half = a.bn >> 1;
+        int col;
+        if (kMode == kGate) col = rank * a.inter + t.n0 * half;
+        else col = t.n0 * a.bn + rank * half;
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!ptx::mbar_wait(&ctl.empty[slot], phase ^ 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t sa = ptx::smem_u32(smem + slot * kStageBytes), sb = sa + kABytes;
+          const uint32_t bar = map_rank(&ctl.full[slot], 0);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[slot], a.tx_bytes);
+          if (kAMn) {
+            tma_pair(sa, &map_a, row, kb * kBk, bar);
+            tma_pair(sa + 8192, &map_a, row + 64, kb * kBk, bar);
+          } else {
+            tma_pair(sa, &map_a, kb * kBk, row, bar);
+          }
+          if (kBMn) {
+            tma_pair(sb, &map_b, col, kb * kBk, bar);
+            if (half > 64) tma_pair(sb + 8192, &map_b, col + 64, kb * kBk, bar);
+          } else {
+            tma_pair(sb, &map_b, kb * kBk, col, bar);
+          }
+          if (++slot == kStages) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // the commits that free the last stages arrive here too: see them land before leaving
+      for (int s = 0; s < kStages && ok; ++s) {
+        if (!ptx::mbar_wait(&ctl.empty[slot], phase ^ 1)) ok = false;
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && ptx::elect_one()) {
+      int slot = 0, it = 0;
+      uint32_t phase = 0;
+      for (int w = pair; w < total && ok; w += pairs, ++it) {
+        const Tile t = tile_of(a, w);
+        const int buf = it & 1;
+        if (!ptx::mbar_wait(&ctl.acc_empty[buf], ((it >> 1) & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + buf * kMaxBn;
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!ptx::mbar_wait(&ctl.full[slot], phase)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t sa = ptx::smem_u32(smem + slot * kStageBytes);
+          const uint64_t da = operand_desc<kAMn>(sa), db = operand_desc<kBMn>(sa + kABytes);
+#pragma unroll
+          for (int j = 0; j < kBk / 16; ++j)
+            mma_pair(d, da + j * kStepDesc<kAMn>, db + j * kStepDesc<kBMn>, a.idesc, kb > t.kb0 || j > 0);
+          commit_pair(&ctl.empty[slot]);
+          if (++slot == kStages) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+        commit_pair(&ctl.acc_full[buf]);
+      }
+    }
+  } else {
+    const int e = warp - 2, quarter = warp & 3, half = e >> 2;
+    uint8_t* patch = patches + e * kPatch;
+    const uint32_t lane_base = tmem + ((uint32_t)quarter << 21);
+    const int rr = lane >> 3, cc = (lane & 7) * 4;
+    int it = 0;
+    for (int w = pair; w < total; w += pairs, ++it) {
+      const Tile t = tile_of(a, w);
+      const int buf = it & 1;
+      if (!ptx::mbar_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t acc = lane_base + buf * kMaxBn;
+      const int row0 = t.m0 + rank * kBm + quarter * 32;
+      const bool rows = row0 < a.m;        // a warp whose rows all lie past the end stores nothing
+      // rows 4 i + rr of the patch, columns cc .. cc + 3, for every i whose row exists
+      auto each = [&](const float (&v)[32], auto&& f) {
+        __syncwarp();
+        patch_put(patch, lane, v);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (row0 + 4 * i + rr < a.m) f(row0 + 4 * i + rr, patch_get(patch, lane, i));
+      };
+      if (rows && kMode == kGate) {
+        const int pairs_cols = a.bn >> 1;  // gate columns of the tile; the up columns follow
+        for (int c = 32 * half; c < pairs_cols; c += 64) {
+          const int col = t.n0 * pairs_cols + c + cc;
+          if (t.n0 * pairs_cols + c >= a.inter) break;
+          float g[32], u[32];
+          tmem_ld32(acc + c, g);
+          tmem_ld32(acc + pairs_cols + c, u);
+          ptx::tmem_wait_ld();
+          const bool in = col < a.inter;
+          if (a.partial || a.ab) {
+            float* to = a.partial ? a.partials + (size_t)t.split * a.m * a.n : a.ab;
+            each(g, [&](int r, float4 v) {
+              if (in) *reinterpret_cast<float4*>(to + (size_t)r * a.n + col) = v;
+            });
+            each(u, [&](int r, float4 v) {
+              if (in) *reinterpret_cast<float4*>(to + (size_t)r * a.n + a.inter + col) = v;
+            });
+          }
+          if (!a.partial) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) g[j] = silu_f(g[j]) * u[j];
+            each(g, [&](int r, float4 v) {
+              if (in) store4(a.dtype, a.out, a.ldo, r, col, v);
+            });
+          }
+        }
+      } else if (rows) {
+        for (int c = 32 * half; c < a.bn; c += 64) {
+          const int col = t.n0 * a.bn + c + cc;
+          if (t.n0 * a.bn + c >= a.n) break;
+          const bool in = col < a.n;
+          float4 ga[8], gb[8];
+          if (kMode == kDGate && !a.partial) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (in && row0 + 4 * i + rr < a.m) {
+                const float* at = a.ab + (size_t)(row0 + 4 * i + rr) * 2 * a.inter + col;
+                ga[i] = __ldg(reinterpret_cast<const float4*>(at));
+                gb[i] = __ldg(reinterpret_cast<const float4*>(at + a.inter));
+              }
+          }
+          float v[32];
+          tmem_ld32(acc + c, v);
+          ptx::tmem_wait_ld();
+          __syncwarp();
+          patch_put(patch, lane, v);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = row0 + 4 * i + rr;
+            if (!in || r >= a.m) continue;
+            float4 x = patch_get(patch, lane, i);
+            if (a.partial) {
+              *reinterpret_cast<float4*>(a.partials + ((size_t)t.split * a.m + r) * a.n + col) = x;
+            } else if (kMode == kDGate) {
+              dgate4(a, r, col, x, ga[i], gb[i]);
+            } else {
+              if (a.add) x = add4(a.dtype, a.add, a.ld_add, r, col, x);
+              store4(a.dtype, a.out, a.ldo, r, col, x);
+            }
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(map_rank(&ctl.acc_empty[buf], 0));
+    }
+  }
+  if (!ok) {
+    // An expired wait: report it, and leave copies and MMAs in flight time to land before the
+    // shared and tensor memory go.
+    if (a.error_flag) atomicExch(a.error_flag, kWaitFailed);
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000LL) __nanosleep(1000);
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
+  ptx::tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Sum of the splits' partials, in split order, with the mode's epilogue. One float4 of columns
+// per thread; the partials were just written and are read from L2.
+template <int kMode>
+__global__ void __launch_bounds__(256) dense_reduce(const Args a) {
+  chain_release();
+  chain_wait();
+  const int width = kMode == kGate ? a.inter : a.n;
+  const int q = width >> 2;
+  const size_t plane = (size_t)a.m * a.n;
+  const size_t items = (size_t)a.m * q;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < items; i += (size_t)gridDim.x * blockDim.x) {
+    const int row = (int)(i / q), col = (int)(i - (size_t)row * q) * 4;
+    auto sum = [&](int c) {
+      const float* p = a.partials + (size_t)row * a.n + c;
+      float4 s = __ldcg(reinterpret_cast<const float4*>(p));
+#pragma unroll 4
+      for (int k = 1; k < a.splits; ++k) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + k * plane));
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+      return s;
+    };
+    float4 x = sum(col);
+    if (kMode == kGate) {
+      const float4 u = sum(a.inter + col);
+      if (a.ab) {
+        float* at = a.ab + (size_t)row * a.n + col;
+        *reinterpret_cast<float4*>(at) = x;
+        *reinterpret_cast<float4*>(at + a.inter) = u;
+      }
+      x = make_float4(silu_f(x.x) * u.x, silu_f(x.y) * u.y, silu_f(x.z) * u.z, silu_f(x.w) * u.w);
+      store4(a.dtype, a.out, a.ldo, row, col, x);
+    } else if (kMode == kDGate) {
+      const float* at = a.ab + (size_t)row * 2 * a.inter + col;
+      dgate4(a, row, col, x, __ldg(reinterpret_cast<const float4*>(at)),
+             __ldg(reinterpret_cast<const float4*>(at + a.inter)));
+    } else {
+      if (a.add) x = add4(a.dtype, a.add, a.ld_add, row, col, x);
+      store4(a.dtype, a.out, a.ldo, row, col, x);
+    }
+  }
+}
+
+constexpr int kPairs = 74;  // 148 SMs, two to a pair
+
+struct Plan {
+  int bn, tiles_m, tiles_n, splits, kb_total, kb_per_split;
+};
+
+// Tile width and split of K, from the sizes alone: the least estimated time in SM clocks. A stage
+// of a pair costs the larger of its MMA time (2 bn clocks for 64 k) and its loads ((128 + bn / 2)
+// rows of 128 B at ~60 B per clock and SM from L2); a tile's start and last epilogue ~2500; a split adds the
+// reduction's launch and its partials' way through L2 (~2 KB per clock over the chip).
+Plan make_plan(int m, int n, int k, int mode, bool b_k_major) {
+  Plan best{};
+  double best_cost = 0;
+  const int kb = (k + kBk - 1) / kBk;
+  for (int bn = 256; bn >= 64; bn -= 32) {
+    if (!b_k_major && bn != 256 && bn != 128) continue;
+    if (mode == kGate && bn % 64) continue;
+    Plan p;
+    p.bn = bn;
+    p.tiles_m = (m + 2 * kBm - 1) / (2 * kBm);
+    p.tiles_n = (n + bn - 1) / bn;
+    if (mode == kGate) p.tiles_n = (n / 2 + bn / 2 - 1) / (bn / 2);
+    p.kb_total = kb;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    const double stage = 2.0 * bn > (128 + bn / 2) * 128 / 60.0 ? 2.0 * bn : (128 + bn / 2) * 128 / 60.0;
+    for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= kPairs && kb / s >= 4)); ++s) {
+      p.kb_per_split = (kb + s - 1) / s;
+      p.splits = (kb + p.kb_per_split - 1) / p.kb_per_split;
+      const double waves = (double)((tiles * p.splits + kPairs - 1) / kPairs);
+      double cost = waves * p.kb_per_split * stage + 2500;
+      if (p.splits > 1) cost += 4000 + 8.0 * m * n * p.splits / 2000;
+      if (best.bn == 0 || cost < best_cost) {
+        best = p;
+        best_cost = cost;
+      }
+    }
+  }
+  return best;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// Map of an operand with `extent` m (or n) and k: boxes of 64 k x box rows (K-major) or of
+// 64 m x 64 k.
+int make_map(CUtensorMap* map, const DenseOperand& o, int extent, int k, int dtype, int box) {
+  const auto encode = encode_fn();
+  if (!encode) return MUSE_ERR_NO_DEVICE;
+  cuuint64_t dims[2] = {(cuuint64_t)(o.k_major ? k : extent), (cuuint64_t)(o.k_major ? extent : k)};
+  cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
+  cuuint32_t boxes[2] = {64, (cuuint32_t)(o.k_major ? box : 64)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r =
+      encode(map, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(o.ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MUSE_OK : MUSE_ERR_INVALID_ARGUMENT;
+}
+
+template <bool kAMn, bool kBMn, int kMode>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, cudaStream_t st) {
+  // once per device and kernel: the attribute belongs to the device's context
+  static bool set[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev >= 64 || !set[dev]) {
+    e = cudaFuncSetAttribute(dense_gemm<kAMn, kBMn, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 64) set[dev] = true;
+  }
+  const long long total = (long long)a.tiles_m * a.tiles_n * a.splits;
+  const int pairs = total < kPairs ? (int)total : kPairs;
+  int rc = launch_chained(dense_gemm<kAMn, kBMn, kMode>, dim3(2 * pairs), dim3(kThreads), kSmem, st, 2, ma, mb, a);
+  if (rc || !a.partial) return rc;
+  const size_t items = (size_t)a.m * ((kMode == kGate ? a.inter : a.n) >> 2);
+  const size_t blocks = (items + 255) / 256;
+  return launch_chained(dense_reduce<kMode>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st,
+                        1, a);
+}
+
+}  // namespace
+
+size_t dense_scratch_bytes(int m, int n, int k, int mode, bool b_k_major) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const Plan p = make_plan(m, n, k, mode, b_k_major);
+  return p.splits > 1 ? (size_t)4 * p.splits * m * n : 0;
+}
+
+int launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
+  const Plan p = make_plan(g.m, g.n, g.k, g.mode, g.b.k_major);
+  if ((long long)p.tiles_m * p.tiles_n * p.splits > 0x7FFFFFFFLL) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  Args a{};
+  a.m = g.m;
+  a.n = g.n;
+  a.inter = g.mode == kGate ? g.n / 2 : g.mode == kDGate ? g.n : 0;
+  a.bn = p.bn;
+  a.tiles_m = p.tiles_m;
+  a.tiles_n = p.tiles_n;
+  a.splits = p.splits;
+  a.kb_total = p.kb_total;
+  a.kb_per_split = p.kb_per_split;
+  a.dtype = g.dtype;
+  a.partial = p.splits > 1;
+  const uint32_t type = g.dtype == kBf16 ? 1u : 0u;  // operand format: 0 f16, 1 bf16
+  a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((g.a.k_major ? 0u : 1u) << 15) |
+            ((g.b.k_major ? 0u : 1u) << 16) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(2 * kBm >> 4) << 24);
+  a.tx_bytes = 2 * (kABytes + (uint32_t)p.bn / 2 * kBk * 2);
+  a.out = g.out;
+  a.ldo = g.ldo;
+  a.add = g.add;
+  a.ld_add = g.ld_add;
+  a.ab = g.ab;
+  a.h_out = g.h_out;
+  a.partials = g.partials;
+  a.error_flag = g.error_flag;
+  if (a.partial && !g.partials) return MUSE_ERR_WORKSPACE_TOO_SMALL;
+  CUtensorMap ma, mb;
+  int rc = make_map(&ma, g.a, g.m, g.k, g.dtype, kBm);
+  if (!rc) rc = make_map(&mb, g.b, g.n, g.k, g.dtype, p.bn / 2);
+  if (rc) return rc;
+  if (g.a.k_major && g.b.k_major) {
+    if (g.mode == kGate) return launch<false, false, kGate>(ma, mb, a, stream);
+    if (g.mode == kStore) return launch<false, false, kStore>(ma, mb, a, stream);
+  } else if (g.a.k_major) {
+    if (g.mode == kDGate) return launch<false, true, kDGate>(ma, mb, a, stream);
+    if (g.mode == kStore) return launch<false, true, kStore>(ma, mb, a, stream);
+  } else if (!g.b.k_major && g.mode == kStore) {
+    return launch<true, true, kStore>(ma, mb, a, stream);
+  }
+  return MUSE_ERR_INVALID_ARGUMENT;
+}
+
+}  // namespace muse

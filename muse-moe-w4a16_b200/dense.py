@@ -1,0 +1,225 @@
+"""Dense products beside the routed experts: linear_w4 (NVFP4 weights) and gated_ffn (16-bit
+weights, with gradients).
+
+Both are what a layer with routed experts needs next to them: its dense projections and its
+shared expert, whose output is added to the routed one (`add`). Same rules as kernel_fn: CUDA
+tensors only, the current stream, memory from torch's caching allocator, no host
+synchronisation; so calls can be captured in a CUDA graph after one eager call.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import functools
+from typing import TypedDict
+
+import torch
+
+from . import _lib
+from .layer import _require_cuda, _stream
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+class LinearWeights(TypedDict):
+    w: torch.Tensor      # uint8 [N, K/2], packed E2M1, element 2i in the low nibble
+    w_sf: torch.Tensor   # float8_e4m3fn [N, K/16]
+    w_gs: torch.Tensor   # float32, one element
+
+
+def _bad(message: str) -> _lib.MuseError:
+    return _lib.MuseError(_lib.MUSE_ERR_INVALID_ARGUMENT, message)
+
+
+def _on(device: torch.device):
+    """Context with `device` current (the kernels launch on the current device)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _same(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) -> None:
+    if t.device != device:
+        raise _bad(f"{name} is on {t.device}, x on {device}")
+    if t.dtype != dtype:
+        raise _bad(f"{name} is {t.dtype}, x {dtype}")
+
+
+def _rows(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
+    """`t` [..., width] as 16-byte aligned rows and their stride: in place where its strides
+    allow it, else a contiguous copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    ld = t.stride(0) if t.shape[0] > 1 else width
+    if t.stride(1) != 1 or ld % 8 or ld < width or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        ld = width
+    return t, ld
+
+
+def prepare_linear(weight: LinearWeights, gated: bool = False) -> dict:
+    """Repack an NVFP4 matrix [N, K] for linear_w4 (once, untimed): any N, K a multiple of 16.
+    gated: rows [0, N/2) are gate rows and the rest the matching up rows (a w13)."""
+    w, sf, gs = weight["w"], weight["w_sf"], weight["w_gs"]
+    _require_cuda(w, "w")
+    if w.dtype != torch.uint8 or w.dim() != 2 or 0 in w.shape:
+        raise _bad("w must be a uint8 matrix of packed codes [N, K/2]")
+    N, K = w.shape[0], 2 * w.shape[1]
+    if K % 16:
+        raise _bad(f"K = {K} is not a multiple of 16")
+    if gated and N % 2:
+        raise _bad(f"a gated weight has gate and up rows in equal number, got {N} rows")
+    if sf.dtype not in (torch.float8_e4m3fn, torch.uint8) or tuple(sf.shape) != (N, K // 16):
+        raise _bad(f"w_sf must be float8_e4m3fn {(N, K // 16)}, got {sf.dtype} {tuple(sf.shape)}")
+    if gs.numel() != 1 or not gs.is_floating_point():
+        raise _bad("w_gs must be one floating-point value")
+    dev = w.device
+    if sf.device != dev:
+        raise _bad(f"w_sf is on {sf.device}, w on {dev}")
+    codes, scales = w.contiguous(), sf.contiguous().view(torch.uint8)
+    if codes.data_ptr() % 8:
+        codes = codes.clone()
+    nc, ns = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _lib.call("muse_moe_linear_prepared_size", N, K, int(gated), ctypes.byref(nc), ctypes.byref(ns))
+    out = torch.empty(nc.value, dtype=torch.uint8, device=dev)
+    out_sf = torch.empty(ns.value, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.call("muse_moe_prepare_linear", codes.data_ptr(), scales.data_ptr(), N, K, int(gated),
+                  out.data_ptr(), out_sf.data_ptr(), _stream(dev))
+    return {"w": out, "w_sf": out_sf, "w_gs": gs.to(device=dev, dtype=torch.float32).reshape(1).clone(),
+            "rows": N, "cols": K, "gated": bool(gated), "n_out": N // 2 if gated else N}
+
+
+def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """x [..., K] times a prepared NVFP4 matrix: [..., N], or silu(gate) * up [..., N/2] for a gated
+    one, plus `add` (same shape) if given. x is bf16 or fp16, and so are add and the result; any
+    number of rows. Sums in fp32, one rounding. Inference only: it has no gradient."""
+    _require_cuda(x, "x")
+    K, n_out, dev = state["cols"], state["n_out"], x.device
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
+        raise _bad(f"x must be bfloat16 or float16, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise _bad(f"x {tuple(x.shape)} does not end in the weight's {K} columns")
+    if state["w"].device != dev:
+        raise _bad(f"the weight is on {state['w'].device}, x on {dev}")
+    if torch.is_grad_enabled() and (x.requires_grad or (add is not None and add.requires_grad)):
+        raise _bad("linear_w4 has no gradient: call it under torch.no_grad()")
+    shape = x.shape[:-1] + (n_out,)
+    x2, ldx = _rows(x, K)
+    T = x2.shape[0]
+    add_ptr, ld_add = None, 0
+    if add is not None:
+        _same(add, "add", dev, x.dtype)
+        if add.shape != shape:
+            raise _bad(f"add must be {tuple(shape)}, got {tuple(add.shape)}")
+        add2 = add if add.dim() == 2 else add.reshape(-1, n_out)
+        if add2.stride(1) != 1 or (T > 1 and add2.stride(0) < n_out):
+            add2 = add2.contiguous()
+        add_ptr, ld_add = add2.data_ptr(), add2.stride(0)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
+        raise _bad(f"out must be a contiguous {x.dtype} {tuple(shape)} on {dev}")
+    with _on(dev):
+        _lib.call("muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, int(state["gated"]),
+                  state["w"].data_ptr(), state["w_sf"].data_ptr(), state["w_gs"].data_ptr(), add_ptr, ld_add,
+                  out.data_ptr(), n_out, _stream(dev))
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _ffn_workspace(tokens: int, hidden: int, inter: int, backward: int) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.call("muse_moe_ffn_workspace_size", tokens, hidden, inter, backward, ctypes.byref(n))
+    return n.value
+
+
+def _ffn_forward(x, w13, w2, add, keep: bool):
+    """(out, ab): the block's output and, with `keep`, its fp32 pre-activations [T, 2I]."""
+    H, I = w2.shape
+    dev, dtype = x.device, x.dtype
+    x2, ldx = _rows(x, H)
+    T = x2.shape[0]
+    out = torch.empty(x.shape, dtype=dtype, device=dev)
+    ab = torch.empty((T, 2 * I), dtype=torch.float32, device=dev) if keep else None
+    if T == 0:
+        return out, ab
+    w13, ld13 = _rows(w13, H)
+    w2, ld2 = _rows(w2, I)
+    add2, ld_add = (None, 0) if add is None else _rows(add, H)
+    n = _ffn_workspace(T, H, I, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.call("muse_moe_ffn_forward", x2.data_ptr(), ldx, _DTYPES[dtype], T, H, I, w13.data_ptr(), ld13,
+                  w2.data_ptr(), ld2, None if add is None else add2.data_ptr(), ld_add, out.data_ptr(),
+                  ab.data_ptr() if keep else None, ws.data_ptr(), n, _stream(dev))
+    return out, ab
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, w2, add):
+        keep = any(ctx.needs_input_grad[:3])
+        out, ab = _ffn_forward(x, w13, w2, add, keep)
+        if keep:
+            ctx.save_for_backward(x, w13, w2, ab)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_x, need_13, need_2, need_add = ctx.needs_input_grad
+        dx = dw13 = dw2 = None
+        if need_x or need_13 or need_2:
+            x, w13, w2, ab = ctx.saved_tensors
+            H, I = w2.shape
+            T, dev = ab.shape[0], x.device
+            make = torch.zeros if T == 0 else torch.empty
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+            dw13 = make((2 * I, H), dtype=x.dtype, device=dev) if need_13 else None
+            dw2 = make((H, I), dtype=x.dtype, device=dev) if need_2 else None
+            if T:
+                dy2, ldy = _rows(dy, H)
+                x2, ldx = _rows(x, H)
+                w13, ld13 = _rows(w13, H)
+                w2, ld2 = _rows(w2, I)
+                n = _ffn_workspace(T, H, I, 1)
+                ws = torch.empty(n, dtype=torch.uint8, device=dev)
+                with _on(dev):
+                    _lib.call("muse_moe_ffn_backward", dy2.data_ptr(), ldy, x2.data_ptr(), ldx, _DTYPES[x.dtype], T,
+                              H, I, w13.data_ptr(), ld13, w2.data_ptr(), ld2, ab.data_ptr(),
+                              dx.data_ptr() if need_x else None, dw13.data_ptr() if need_13 else None,
+                              dw2.data_ptr() if need_2 else None, ws.data_ptr(), n, _stream(dev))
+        return dx, dw13, dw2, dy if need_add else None
+
+
+def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, add: torch.Tensor | None = None) -> torch.Tensor:
+    """The gated feed-forward block (silu(x Wg^T) * (x Wu^T)) W2^T (+ add), 16-bit weights.
+
+    x [..., H], w13 [2I, H] (gate rows, then up rows, as the routed experts' w13), w2 [H, I], add of
+    x's shape; all bf16 or all fp16; H and I multiples of 8. Differentiable in every tensor. A
+    pass that needs gradients keeps the pre-activations in fp32 (8 T I bytes)."""
+    _require_cuda(x, "x")
+    dev = x.device
+    if x.dtype not in _DTYPES:
+        raise _bad(f"x must be bfloat16 or float16, got {x.dtype}")
+    _same(w13, "w13", dev, x.dtype)
+    _same(w2, "w2", dev, x.dtype)
+    if w13.dim() != 2 or w2.dim() != 2 or x.dim() == 0:
+        raise _bad("gated_ffn needs x [..., H], w13 [2I, H] and w2 [H, I]")
+    H, I = w2.shape
+    if x.shape[-1] != H or tuple(w13.shape) != (2 * I, H):
+        raise _bad(f"inconsistent shapes: x {tuple(x.shape)}, w13 {tuple(w13.shape)}, w2 {tuple(w2.shape)}")
+    if H == 0 or I == 0 or H % 8 or I % 8:
+        raise _lib.MuseError(_lib.MUSE_ERR_UNSUPPORTED_SHAPE, f"H = {H} and I = {I} must be multiples of 8")
+    if add is not None:
+        _same(add, "add", dev, x.dtype)
+        if add.shape != x.shape:
+            raise _bad(f"add must be {tuple(x.shape)}, got {tuple(add.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad
+                                    or (add is not None and add.requires_grad)):
+        return _GatedFfn.apply(x, w13, w2, add)
+    return _ffn_forward(x, w13, w2, add, False)[0]
