@@ -2,6 +2,7 @@
 // feed-forward block's forward and backward products.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -49,6 +50,10 @@ struct DenseGemm {
 // Scratch bytes of the fp32 partial sums for these sizes (0: K is not split).
 size_t dense_scratch_bytes(int m, int n, int k, int mode, bool b_k_major);
 int launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
+
+// Tensor map of an operand with `extent` m (or n) and k: boxes of 64 k x box rows (K-major) or of
+// 64 m x 64 k, 128-byte swizzle, zeros out of bounds.
+int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k, int dtype, int box);
 
 // ---- 16-bit conversions shared by the dense kernels
 

@@ -25,7 +25,7 @@
 #include <cudaTypedefs.h>
 
 #include "kernels.cuh"
-#include "ptx.cuh"
+#include "pair.cuh"
 
 namespace muse {
 namespace {
@@ -41,7 +41,6 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kPatch = 32 * 32 * 4;       // one epilogue warp's 32 x 32 fp32 staging patch
 constexpr int kGroupM = 8;                // row tiles per raster group
-constexpr int kWaitFailed = 8;            // device status of an expired wait here
 
 struct Ctl {
   uint64_t full[kStages], empty[kStages];
@@ -66,74 +65,6 @@ struct Args {
   float* partials;
   int* error_flag;
 };
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-// Address of the same shared-memory object in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(ptx::smem_u32(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// TMA box into this CTA's shared memory, completing on a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-// Arrive on `bar` of both CTAs once this thread's MMAs so far have completed.
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          ptx::smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-
-// Shared-memory descriptors, 128-byte swizzle. K-major: rows of 64 k, 8-row groups 1024 B apart.
-// MN-major: boxes of 64 (m or n) x 64 k, 8192 B apart (the leading offset); 8-k groups 1024 B
-// apart (the stride offset).
-template <bool kMn>
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
-  uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)((kMn ? 8192u : 16u) >> 4) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-// Descriptor step of 16 k (in 16-byte units).
-template <bool kMn>
-constexpr uint32_t kStepDesc = kMn ? 16 * 128 / 16 : 2;
 
 struct Tile {
   int m0, n0, kb0, kb1, split;
@@ -412,13 +343,7 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
       if (lane == 0) arrive_cluster(map_rank(&ctl.acc_empty[buf], 0));
     }
   }
-  if (!ok) {
-    // An expired wait: report it, and leave copies and MMAs in flight time to land before the
-    // shared and tensor memory go.
-    if (a.error_flag) atomicExch(a.error_flag, kWaitFailed);
-    const long long t0 = clock64();
-    while (clock64() - t0 < 20000000LL) __nanosleep(1000);
-  }
+  if (!ok) give_up(a.error_flag);
   __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
@@ -511,34 +436,6 @@ Plan make_plan(int m, int n, int k, int mode, bool b_k_major) {
   return best;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  }();
-  return fn;
-}
-
-// Map of an operand with `extent` m (or n) and k: boxes of 64 k x box rows (K-major) or of
-// 64 m x 64 k.
-int make_map(CUtensorMap* map, const DenseOperand& o, int extent, int k, int dtype, int box) {
-  const auto encode = encode_fn();
-  if (!encode) return MUSE_ERR_NO_DEVICE;
-  cuuint64_t dims[2] = {(cuuint64_t)(o.k_major ? k : extent), (cuuint64_t)(o.k_major ? extent : k)};
-  cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
-  cuuint32_t boxes[2] = {64, (cuuint32_t)(o.k_major ? box : 64)};
-  cuuint32_t estr[2] = {1, 1};
-  const CUresult r =
-      encode(map, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-             const_cast<void*>(o.ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? MUSE_OK : MUSE_ERR_INVALID_ARGUMENT;
-}
-
 template <bool kAMn, bool kBMn, int kMode>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, cudaStream_t st) {
   // once per device and kernel: the attribute belongs to the device's context
@@ -562,6 +459,34 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, cudaStre
 }
 
 }  // namespace
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// Map of an operand with `extent` m (or n) and k: boxes of 64 k x box rows (K-major) or of
+// 64 m x 64 k.
+int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k, int dtype, int box) {
+  const auto encode = encode_fn();
+  if (!encode) return MUSE_ERR_NO_DEVICE;
+  cuuint64_t dims[2] = {(cuuint64_t)(o.k_major ? k : extent), (cuuint64_t)(o.k_major ? extent : k)};
+  cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
+  cuuint32_t boxes[2] = {64, (cuuint32_t)(o.k_major ? box : 64)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r =
+      encode(map, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(o.ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MUSE_OK : MUSE_ERR_INVALID_ARGUMENT;
+}
 
 size_t dense_scratch_bytes(int m, int n, int k, int mode, bool b_k_major) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
@@ -598,8 +523,8 @@ int launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
   a.error_flag = g.error_flag;
   if (a.partial && !g.partials) return MUSE_ERR_WORKSPACE_TOO_SMALL;
   CUtensorMap ma, mb;
-  int rc = make_map(&ma, g.a, g.m, g.k, g.dtype, kBm);
-  if (!rc) rc = make_map(&mb, g.b, g.n, g.k, g.dtype, p.bn / 2);
+  int rc = make_operand_map(&ma, g.a, g.m, g.k, g.dtype, kBm);
+  if (!rc) rc = make_operand_map(&mb, g.b, g.n, g.k, g.dtype, p.bn / 2);
   if (rc) return rc;
   if (g.a.k_major && g.b.k_major) {
     if (g.mode == kGate) return launch<false, false, kGate>(ma, mb, a, stream);

@@ -8,13 +8,8 @@
 // codes), the routed experts' own format, so that sixteen rows of a 128-code chunk are 1 KiB in
 // a row and a code pair drops into a bf16x2 with one logic op.
 #undef MUSE_TRACE  // these kernels record no stamps
-#include "dense.cuh"
-
-#include <cuda_fp16.h>
-
 #include "kernels.cuh"
-#include "layout.cuh"
-#include "ptx.cuh"
+#include "w4.cuh"
 
 namespace muse {
 namespace {
@@ -71,56 +66,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t mul2_bf16(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t mul2_f16(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-
-// Two e4m3 scales -> a pair register per scale. bf16: (s * 2^118, twice); fp16: (s * 2^5, twice).
-// Exact: four significant bits, and 448 * 2^118 and 448 * 2^5 are in range.
-template <bool kHalf>
-__device__ __forceinline__ void expand_scales(uint32_t two, uint32_t& s0, uint32_t& s1) {
-  uint32_t h;
-  asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(two));
-  if (kHalf) {
-    const uint32_t v = mul2_f16(h, 0x50005000u);  // 2^5
-    s0 = __byte_perm(v, v, 0x1010);
-    s1 = __byte_perm(v, v, 0x3232);
-  } else {
-    const float2 f = unpack16(kFp16, h);
-    constexpr float kUp = 332306998946228968225951765070086144.0f;  // 2^118
-    s0 = pack16(kBf16, f.x * kUp, f.x * kUp);
-    s1 = pack16(kBf16, f.y * kUp, f.y * kUp);
-  }
-}
-
-// One permuted code word -> four pairs (natural element order) times the scale register.
-// The masked bits read as bf16 are e2m1 * 2^-126; with the scale the result is e2m1 * e4m3 * 2^-8,
-// six significant bits: exact. For fp16 the three magnitude bits move up by three (e2m1 * 2^-14);
-// times s * 2^5, then times 2^9: e2m1 * e4m3, exact (every step is a multiple of 2^-24).
-template <bool kHalf>
-__device__ __forceinline__ void dequant_word(uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
-  constexpr uint32_t kMask = 0x81C081C0u;
-  uint32_t v[4] = {w & kMask, ptx::rotl(w, 4) & kMask, ptx::rotl(w, 10) & kMask,
-                   ((w << 6) & 0x80C080C0u) | ((w >> 2) & 0x01000100u)};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (kHalf) {
-      const uint32_t u = (v[i] & 0x80008000u) | ((v[i] << 3) & 0x0E000E00u);
-      out[i] = mul2_f16(mul2_f16(u, scale), 0x60006000u);  // 2^9
-    } else {
-      out[i] = mul2_bf16(v[i], scale);
-    }
-  }
-}
-template <bool kHalf> constexpr float kUnscale = kHalf ? 1.f : 256.f;
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -130,27 +75,6 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 constexpr int kFewWarps = 8;
 // Chunks in flight per warp: the token rows share the ring, so more tokens leave room for fewer.
 template <int kNT> constexpr int kDepthOf = kNT == 1 ? 4 : kNT == 2 ? 3 : 2;
-
-struct LinearArgs {
-  const uint8_t* wq;
-  const uint8_t* wsf;
-  const float* gs;
-  const uint16_t* x;
-  long long ldx;
-  const uint16_t* add;
-  long long ld_add;
-  uint16_t* out;
-  long long ldo;
-  int tokens, cols, n_out;   // n_out: columns of y
-  int k_chunks;
-  int tile_tokens;           // tokens per CTA (x staging rows)
-};
-
-__device__ __forceinline__ float load16(int dtype, const uint16_t* p) {
-  const uint16_t v = __ldg(p);
-  return dtype == kBf16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
-}
-__device__ __forceinline__ uint16_t round16(int dtype, float v) { return (uint16_t)(pack16(dtype, v, v) & 0xFFFF); }
 
 // A CTA of eight warps computes 16 * kMT weight rows for up to 8 * kNT tokens; the warps take the
 // 128-code chunks of K in turn and a cluster of CTAs splits them further, so that a matrix of few
@@ -328,9 +252,9 @@ linear_few(const LinearArgs a) {
 }
 
 template <int kMT, int kNT, bool kHalf, bool kGated>
-int launch_few(LinearArgs a, int padded_rows, cudaStream_t st) {
+int launch_few(LinearArgs a, cudaStream_t st) {
   a.tile_tokens = a.tokens < 8 * kNT ? a.tokens : 8 * kNT;
-  const int ctas = padded_rows / (16 * kMT);
+  const int ctas = a.padded_rows / (16 * kMT);
   const int y = (a.tokens + a.tile_tokens - 1) / a.tile_tokens;
   int cluster = 1;
   while (cluster < 8 && (long long)ctas * y * cluster < 2 * 148 && a.k_chunks >= 2 * kFewWarps * cluster) cluster *= 2;
@@ -351,13 +275,16 @@ int launch_few(LinearArgs a, int padded_rows, cudaStream_t st) {
 }
 
 template <int kMT, int kNT>
-int launch_few_typed(const LinearArgs& a, int padded_rows, int dtype, bool gated, cudaStream_t st) {
+int launch_few_typed(const LinearArgs& a, int dtype, bool gated, cudaStream_t st) {
   if (gated)
-    return dtype == kFp16 ? launch_few<(kMT < 2 ? 2 : kMT), kNT, true, true>(a, padded_rows, st)
-                          : launch_few<(kMT < 2 ? 2 : kMT), kNT, false, true>(a, padded_rows, st);
-  return dtype == kFp16 ? launch_few<kMT, kNT, true, false>(a, padded_rows, st)
-                        : launch_few<kMT, kNT, false, false>(a, padded_rows, st);
+    return dtype == kFp16 ? launch_few<(kMT < 2 ? 2 : kMT), kNT, true, true>(a, st)
+                          : launch_few<(kMT < 2 ? 2 : kMT), kNT, false, true>(a, st);
+  return dtype == kFp16 ? launch_few<kMT, kNT, true, false>(a, st)
+                        : launch_few<kMT, kNT, false, false>(a, st);
 }
+
+// Up to this many tokens the mma.sync kernel streams the weights; beyond, the tcgen05 kernel.
+constexpr int kFewTokens = 8;
 
 int padded(int v, int to) { return (v + to - 1) / to * to; }
 
@@ -398,10 +325,22 @@ extern "C" int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, in
   return last_launch_status();
 }
 
+extern "C" int muse_moe_linear_workspace_size(int tokens, int rows, int cols, int gated, size_t* bytes) {
+  if (!bytes) return MUSE_ERR_INVALID_ARGUMENT;
+  const int rc = check_linear(rows, cols, gated);
+  if (rc) return rc;
+  if (tokens < 0) return MUSE_ERR_INVALID_ARGUMENT;
+  *bytes = tokens > kFewTokens
+               ? linear_gemm_scratch_bytes(tokens, padded_rows_of(rows, gated), padded(cols, kChunkK) / kChunkK)
+               : 0;
+  return MUSE_OK;
+}
+
 extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int rows, int cols, int gated,
                                   const uint8_t* wp, const uint8_t* w_sfp, const float* w_gs, const void* add,
-                                  long long ld_add, void* out, long long ldo, muse_stream_t stream) {
-  const int rc = check_linear(rows, cols, gated);
+                                  long long ld_add, void* out, long long ldo, void* workspace,
+                                  size_t workspace_bytes, muse_stream_t stream) {
+  int rc = check_linear(rows, cols, gated);
   if (rc) return rc;
   const int n_out = gated ? rows / 2 : rows;
   if (tokens < 0 || (dtype != kBf16 && dtype != kFp16)) return MUSE_ERR_INVALID_ARGUMENT;
@@ -423,11 +362,14 @@ extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int t
   a.cols = cols;
   a.n_out = n_out;
   a.k_chunks = padded(cols, kChunkK) / kChunkK;
-  const int pr = padded_rows_of(rows, gated);
+  a.padded_rows = padded_rows_of(rows, gated);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (tokens <= 4) return launch_few_typed<1, 1>(a, pr, dtype, gated, st);
-  if (tokens <= 8) return launch_few_typed<2, 1>(a, pr, dtype, gated, st);
-  if (tokens <= 16) return launch_few_typed<4, 2>(a, pr, dtype, gated, st);
-  if (tokens > 65535 * 32) return MUSE_ERR_UNSUPPORTED_SHAPE;
-  return launch_few_typed<4, 4>(a, pr, dtype, gated, st);
+  if (tokens <= 4) return launch_few_typed<1, 1>(a, dtype, gated, st);
+  if (tokens <= kFewTokens) return launch_few_typed<2, 1>(a, dtype, gated, st);
+  const size_t scratch = linear_gemm_scratch_bytes(tokens, a.padded_rows, a.k_chunks);
+  if (scratch > 0 && (!workspace || misaligned(workspace, 16))) return MUSE_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < scratch) return MUSE_ERR_WORKSPACE_TOO_SMALL;
+  int* flag = nullptr;
+  if ((rc = device_status_ptr(&flag))) return rc;
+  return launch_linear_gemm(a, dtype, gated, static_cast<float*>(workspace), flag, st);
 }

@@ -1,0 +1,417 @@
+// y = x . W^T with a prepared NVFP4 weight for more than a few tokens, on tcgen05 CTA pairs.
+//
+// Swap-AB: 256 weight rows per pair are the MMA's M, up to 256 tokens its N, so a decode batch
+// wastes no rows of M. Per 128-code chunk a CTA copies its 128 rows' codes and scales (9 KiB, one
+// bulk copy each) into a six-deep ring; eight warps turn them into exact 16-bit weights in
+// registers and write them as the K-major swizzled A operand (thread = weight row, one 128-byte
+// row of 64 k each); B is x by TMA, each CTA half of the tokens. Weights are dequantised once per
+// 256 tokens, which at ~140 instructions per thread and 64 k fits under the 512 clocks the MMAs
+// of a 256-token stage take. Accumulators are double buffered in tensor memory; the epilogue's
+// thread is a weight row, so for one token a warp stores 32 neighbouring outputs. A gated tile
+// holds 16 gate and the 16 matching up rows per warp: lanes i and i + 16 swap halves of a token
+// pair by one shuffle.
+// With fewer tiles than pairs K is split; a second kernel adds the fp32 partials in split order.
+// Bound by weight bytes and the dequantisation for tens of tokens, by the tensor pipe for hundreds.
+#undef MUSE_TRACE  // these kernels record no stamps
+#include "kernels.cuh"
+#include "pair.cuh"
+#include "w4.cuh"
+
+namespace muse {
+namespace {
+
+constexpr int kStages = 5;                   // 64-k stages: A (16 KiB) and half of B (16 KiB)
+constexpr int kABytes = kTileM * 128;
+constexpr int kStageBytes = 2 * kABytes;
+constexpr int kCodes = 6;                    // code ring: 128-code chunks of 9 KiB
+constexpr int kCodeBytes = kTileCodeBytes + kTileScaleBytes;
+constexpr int kMaxBn = 256;
+constexpr int kDeqWarp0 = 4, kEpiWarp0 = 12, kThreads = 512;
+
+struct Ctl {
+  uint64_t full[kStages], empty[kStages];
+  uint64_t code_full[kCodes], code_empty[kCodes];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem;
+};
+constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + (size_t)kCodes * kCodeBytes + sizeof(Ctl);
+static_assert(kSmem <= 232448, "shared memory of one CTA");
+
+struct GemmPlan {
+  int bn, tiles_m, tiles_n, splits, chunks_per_split;
+};
+
+struct Args {
+  LinearArgs l;
+  GemmPlan p;
+  uint32_t idesc;
+  uint32_t b_bytes;    // one CTA's B bytes per stage
+  float* partials;     // null: write the outputs
+  int* error_flag;
+};
+
+struct Tile {
+  int m_tile, tok0, c0, c1, split;
+};
+// Work item -> tile: splits innermost, then eight row tiles per token tile.
+__device__ __forceinline__ Tile tile_of(const GemmPlan& p, int k_chunks, int w, uint32_t rank) {
+  constexpr int kGroup = 8;
+  Tile t;
+  const int idx = w / p.splits;
+  t.split = w - idx * p.splits;
+  const int group = idx / (kGroup * p.tiles_n);
+  const int first = group * kGroup;
+  const int rows = min(kGroup, p.tiles_m - first);
+  const int r = idx - group * kGroup * p.tiles_n;
+  t.m_tile = 2 * (first + r % rows) + (int)rank;
+  t.tok0 = r / rows * p.bn;
+  t.c0 = t.split * p.chunks_per_split;
+  t.c1 = min(k_chunks, t.c0 + p.chunks_per_split);
+  return t;
+}
+
+// Position in a ring.
+struct Pos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++slot == size) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+template <bool kHalf, bool kGated>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* codes = smem + kStages * kStageBytes;
+  Ctl& ctl = *reinterpret_cast<Ctl*>(codes + kCodes * kCodeBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int total = a.p.tiles_m * a.p.tiles_n * a.p.splits;
+  const int k_chunks = a.l.k_chunks;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&ctl.full[s], 1 + 2 * 4);  // B bytes announced by the leader; A by four warps of each CTA
+      ptx::mbar_init(&ctl.empty[s], 1);
+    }
+    for (int s = 0; s < kCodes; ++s) {
+      ptx::mbar_init(&ctl.code_full[s], 1);
+      ptx::mbar_init(&ctl.code_empty[s], 8);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(&ctl.acc_full[b], 1);
+      ptx::mbar_init(&ctl.acc_empty[b], 2 * 4);
+    }
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&map_x);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::smem_u32(&ctl.tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = ctl.tmem;
+  chain_release();
+
+  bool ok = true;
+  if (warp == 0) {
+    // Codes: written by prepare only, so they are fetched without waiting for the kernel before.
+    if (ptx::elect_one()) {
+      Pos q;
+      for (int w = pair; w < total && ok; w += pairs) {
+        const Tile t = tile_of(a.p, k_chunks, w, rank);
+        // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
+        const int m = min(t.m_tile, a.l.padded_rows / kTileM - 1);
+        for (int c = t.c0; c < t.c1; ++c) {
+          if (!ptx::mbar_wait_sleep(&ctl.code_empty[q.slot], q.phase ^ 1)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = codes + q.slot * kCodeBytes;
+          const size_t tile = (size_t)m * k_chunks + c;
+          ptx::mbar_arrive_expect_tx(&ctl.code_full[q.slot], kCodeBytes);
+          ptx::bulk_g2s(dst, a.l.wq + tile * kTileCodeBytes, kTileCodeBytes, &ctl.code_full[q.slot]);
+          ptx::bulk_g2s(dst + kTileCodeBytes, a.l.wsf + tile * kTileScaleBytes, kTileScaleBytes, &ctl.code_full[q.slot]);
+          q.next(kCodes);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && ptx::elect_one()) {
+      Pos s;
+      int it = 0;
+      for (int w = pair; w < total && ok; w += pairs, ++it) {
+        const Tile t = tile_of(a.p, k_chunks, w, rank);
+        const int buf = it & 1;
+        if (!ptx::mbar_wait(&ctl.acc_empty[buf], ((it >> 1) & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + buf * kMaxBn;
+        for (int n = 2 * t.c0; n < 2 * t.c1; ++n) {
+          if (!ptx::mbar_wait(&ctl.full[s.slot], s.phase)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t sa = ptx::smem_u32(smem + s.slot * kStageBytes);
+          const uint64_t da = operand_desc<false>(sa), db = operand_desc<false>(sa + kABytes);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, n > 2 * t.c0 || j > 0);
+          commit_pair(&ctl.empty[s.slot]);
+          s.next(kStages);
+        }
+        commit_pair(&ctl.acc_full[buf]);
+      }
+    }
+  } else if (warp == 2) {
+    if (ptx::elect_one()) {
+      chain_wait();
+      Pos s;
+      for (int w = pair; w < total && ok; w += pairs) {
+        const Tile t = tile_of(a.p, k_chunks, w, rank);
+        const int row = t.tok0 + (int)rank * (a.p.bn >> 1);
+        for (int n = 2 * t.c0; n < 2 * t.c1; ++n) {
+          if (!ptx::mbar_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], 2 * a.b_bytes);
+          tma_pair(ptx::smem_u32(smem + s.slot * kStageBytes) + kABytes, &map_x, n * 64, row,
+                   map_rank(&ctl.full[s.slot], 0));
+          s.next(kStages);
+        }
+      }
+      // the commits that free the last stages arrive here too: see them land before leaving
+      for (int i = 0; i < kStages && ok; ++i) {
+        if (!ptx::mbar_wait(&ctl.empty[s.slot], s.phase ^ 1)) ok = false;
+        s.next(kStages);
+      }
+    }
+  } else if (warp >= kDeqWarp0 && warp < kEpiWarp0) {
+    const int h = (warp - kDeqWarp0) >> 2;            // 64-k half of the chunk
+    const int r = (warp & 3) * 32 + lane;             // weight row of the tile
+    Pos q, s;
+    if (h) s.next(kStages);
+    for (int w = pair; w < total && ok; w += pairs) {
+      const Tile t = tile_of(a.p, k_chunks, w, rank);
+      for (int c = t.c0; c < t.c1; ++c) {
+        if (!ptx::mbar_wait_sleep(&ctl.code_full[q.slot], q.phase)) {
+          ok = false;
+          break;
+        }
+        const uint8_t* src = codes + q.slot * kCodeBytes;
+        const uint4 c0 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h));
+        const uint4 c1 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h + 1));
+        const uint32_t sc = *reinterpret_cast<const uint32_t*>(src + kTileCodeBytes + r * kRowScaleBytes + 4 * h);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&ctl.code_empty[q.slot]);
+        uint32_t scale[4];
+        expand_scales<kHalf>(sc & 0xFFFF, scale[0], scale[1]);
+        expand_scales<kHalf>(sc >> 16, scale[2], scale[3]);
+        if (!ptx::mbar_wait_sleep(&ctl.empty[s.slot], s.phase ^ 1)) {
+          ok = false;
+          break;
+        }
+        uint8_t* dst = smem + s.slot * kStageBytes + r * 128;
+        const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t v[4];
+          dequant_word<kHalf>(word[i], scale[i >> 1], v);
+          *reinterpret_cast<uint4*>(dst + ((i ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], 0));
+        q.next(kCodes);
+        s.next(kStages);
+        s.next(kStages);
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    chain_wait();
+    const int quarter = warp & 3;
+    const uint32_t lane_base = tmem + ((uint32_t)quarter << 21);
+    constexpr int dtype = kHalf ? kFp16 : kBf16;
+    const float gs = __ldg(a.l.gs) * kUnscale<kHalf>;
+    int it = 0;
+    for (int w = pair; w < total; w += pairs, ++it) {
+      const Tile t = tile_of(a.p, k_chunks, w, rank);
+      const int buf = it & 1;
+      if (!ptx::mbar_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t acc = lane_base + buf * kMaxBn;
+      const int row = t.m_tile * kTileM + quarter * 32 + lane;   // padded weight row
+      const bool tile_ok = t.m_tile * kTileM < a.l.padded_rows;
+      const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
+      for (int c = 0; c < n_tok && tile_ok; c += 32) {
+        float v[32];
+        tmem_ld32(acc + c, v);
+        ptx::tmem_wait_ld();
+        if (a.partials) {
+          float* to = a.partials + ((size_t)t.split * a.l.tokens + t.tok0 + c) * a.l.padded_rows + row;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < n_tok) to[(size_t)j * a.l.padded_rows] = v[j];
+        } else if (kGated) {
+          // lanes 0-15 take the even token of a pair, 16-31 the odd one
+          const bool upper = lane & 16;
+          const int o = t.m_tile * 64 + quarter * 16 + (lane & 15);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j + 1], 16);
+            const float gate = (upper ? other : v[j]) * gs, up = (upper ? v[j + 1] : other) * gs;
+            const int tok = c + j + (upper ? 1 : 0);
+            if (tok < n_tok && o < a.l.n_out) {
+              float y = silu_f(gate) * up;
+              if (a.l.add) y += load16(dtype, a.l.add + (size_t)(t.tok0 + tok) * a.l.ld_add + o);
+              a.l.out[(size_t)(t.tok0 + tok) * a.l.ldo + o] = round16(dtype, y);
+            }
+          }
+        } else if (row < a.l.n_out) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < n_tok) {
+              float y = v[j] * gs;
+              if (a.l.add) y += load16(dtype, a.l.add + (size_t)(t.tok0 + c + j) * a.l.ld_add + row);
+              a.l.out[(size_t)(t.tok0 + c + j) * a.l.ldo + row] = round16(dtype, y);
+            }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(map_rank(&ctl.acc_empty[buf], 0));
+    }
+  }
+  if (!ok) give_up(a.error_flag);
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
+  ptx::tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Sum of the splits' partials in split order, scale, gate and addend; one output per thread.
+template <bool kHalf, bool kGated>
+__global__ void __launch_bounds__(256) linear_reduce(const Args a) {
+  chain_release();
+  chain_wait();
+  constexpr int dtype = kHalf ? kFp16 : kBf16;
+  const float gs = __ldg(a.l.gs) * kUnscale<kHalf>;
+  const size_t plane = (size_t)a.l.tokens * a.l.padded_rows;
+  const size_t items = (size_t)a.l.tokens * a.l.n_out;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < items; i += (size_t)gridDim.x * blockDim.x) {
+    const int tok = (int)(i / a.l.n_out), o = (int)(i - (size_t)tok * a.l.n_out);
+    const int row = kGated ? (o >> 4) * 32 + (o & 15) : o;
+    const float* p = a.partials + (size_t)tok * a.l.padded_rows + row;
+    float s = 0.f, u = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < a.p.splits; ++k) {
+      s += __ldcg(p + k * plane);
+      if (kGated) u += __ldcg(p + k * plane + 16);
+    }
+    float y = s * gs;
+    if (kGated) y = silu_f(y) * (u * gs);
+    if (a.l.add) y += load16(dtype, a.l.add + (size_t)tok * a.l.ld_add + o);
+    a.l.out[(size_t)tok * a.l.ldo + o] = round16(dtype, y);
+  }
+}
+
+constexpr int kPairs = 74;  // 148 SMs, two to a pair
+
+// Token tile and split of K from the sizes alone: the least estimated time in SM clocks. A 64-k
+// stage costs the most of its MMAs (2 bn), its B rows from L2 (~60 B per clock) and the
+// dequantisation (~190); a tile's start and epilogue 2000 + 8 per token; a split the second
+// kernel's launch and the partials' way through L2 (~2 KB per clock over the chip).
+GemmPlan make_plan(int tokens, int padded_rows, int k_chunks) {
+  GemmPlan best{};
+  double best_cost = 0;
+  for (int bn = 32; bn <= 256; bn += 32) {
+    GemmPlan p;
+    p.bn = bn;
+    p.tiles_m = (padded_rows + 255) / 256;
+    p.tiles_n = (tokens + bn - 1) / bn;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    double stage = 190;
+    if (2.0 * bn > stage) stage = 2.0 * bn;
+    if (bn * 64 / 60.0 > stage) stage = bn * 64 / 60.0;
+    for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= kPairs && k_chunks / s >= 2)); ++s) {
+      p.chunks_per_split = (k_chunks + s - 1) / s;
+      p.splits = (k_chunks + p.chunks_per_split - 1) / p.chunks_per_split;
+      const double waves = (double)((tiles * p.splits + kPairs - 1) / kPairs);
+      double cost = waves * (2 * p.chunks_per_split * stage) + 2000 + 8.0 * bn;
+      if (p.splits > 1) cost += 4000 + 8.0 * tokens * padded_rows * p.splits / 2000;
+      if (best.bn == 0 || cost < best_cost) {
+        best = p;
+        best_cost = cost;
+      }
+    }
+  }
+  return best;
+}
+
+template <bool kHalf, bool kGated>
+int launch(const CUtensorMap& map, const Args& a, cudaStream_t st) {
+  static bool set[64] = {};  // per device: the attribute belongs to its context
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev >= 64 || !set[dev]) {
+    e = cudaFuncSetAttribute(linear_gemm<kHalf, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 64) set[dev] = true;
+  }
+  const long long total = (long long)a.p.tiles_m * a.p.tiles_n * a.p.splits;
+  const int pairs = total < kPairs ? (int)total : kPairs;
+  int rc = launch_chained(linear_gemm<kHalf, kGated>, dim3(2 * pairs), dim3(kThreads), kSmem, st, 2, map, a);
+  if (rc || !a.partials) return rc;
+  const size_t blocks = ((size_t)a.l.tokens * a.l.n_out + 255) / 256;
+  return launch_chained(linear_reduce<kHalf, kGated>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256),
+                        0, st, 1, a);
+}
+
+}  // namespace
+
+size_t linear_gemm_scratch_bytes(int tokens, int padded_rows, int k_chunks) {
+  const GemmPlan p = make_plan(tokens, padded_rows, k_chunks);
+  return p.splits > 1 ? (size_t)4 * p.splits * tokens * padded_rows : 0;
+}
+
+int launch_linear_gemm(const LinearArgs& l, int dtype, bool gated, float* partials, int* error_flag, cudaStream_t st) {
+  Args a{};
+  a.l = l;
+  a.p = make_plan(l.tokens, l.padded_rows, l.k_chunks);
+  if ((long long)a.p.tiles_m * a.p.tiles_n * a.p.splits > 0x7FFFFFFFLL) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  const uint32_t type = dtype == kBf16 ? 1u : 0u;
+  a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(a.p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+  a.b_bytes = (uint32_t)a.p.bn / 2 * 128;
+  a.partials = a.p.splits > 1 ? partials : nullptr;
+  a.error_flag = error_flag;
+  CUtensorMap map;
+  const DenseOperand x{l.x, l.ldx, true};
+  const int rc = make_operand_map(&map, x, l.tokens, l.cols, dtype, a.p.bn / 2);
+  if (rc) return rc;
+  if (dtype == kFp16) return gated ? launch<true, true>(map, a, st) : launch<true, false>(map, a, st);
+  return gated ? launch<false, true>(map, a, st) : launch<false, false>(map, a, st);
+}
+
+}  // namespace muse

@@ -91,6 +91,13 @@ def prepare_linear(weight: LinearWeights, gated: bool = False) -> dict:
             "rows": N, "cols": K, "gated": bool(gated), "n_out": N // 2 if gated else N}
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(tokens: int, rows: int, cols: int, gated: int) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.call("muse_moe_linear_workspace_size", tokens, rows, cols, gated, ctypes.byref(n))
+    return n.value
+
+
 def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] times a prepared NVFP4 matrix: [..., N], or silu(gate) * up [..., N/2] for a gated
@@ -123,10 +130,12 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
         out = torch.empty(shape, dtype=x.dtype, device=dev)
     elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         raise _bad(f"out must be a contiguous {x.dtype} {tuple(shape)} on {dev}")
+    n = _linear_workspace(T, state["rows"], K, int(state["gated"]))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     with _on(dev):
         _lib.call("muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, int(state["gated"]),
                   state["w"].data_ptr(), state["w_sf"].data_ptr(), state["w_gs"].data_ptr(), add_ptr, ld_add,
-                  out.data_ptr(), n_out, _stream(dev))
+                  out.data_ptr(), n_out, ws.data_ptr() if n else None, n, _stream(dev))
     return out
 
 
