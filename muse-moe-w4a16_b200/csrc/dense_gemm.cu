@@ -257,7 +257,7 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
     for (int w = pair; w < total; w += pairs, ++it) {
       const Tile t = tile_of(a, w);
       const int buf = it & 1;
-      if (!ptx::mbar_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
+      if (!warp_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
         ok = false;
         break;
       }

@@ -179,8 +179,8 @@ linear_few(const LinearArgs a) {
         uint32_t lo[4], hi[4];
         const uint32_t wl = j == 0 ? code[m][0].x : j == 1 ? code[m][0].y : j == 2 ? code[m][0].z : code[m][0].w;
         const uint32_t wh = j == 0 ? code[m][1].x : j == 1 ? code[m][1].y : j == 2 ? code[m][1].z : code[m][1].w;
-        dequant_word<kHalf>(wl, sc[m][0][j >> 1], lo);
-        dequant_word<kHalf>(wh, sc[m][1][j >> 1], hi);
+        dequant_word<kHalf>(wl, sc[m][0][j >> 1], a.m16, a.m64, lo);
+        dequant_word<kHalf>(wh, sc[m][1][j >> 1], a.m16, a.m64, hi);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
           mma16816<kHalf>(acc[m][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
@@ -359,6 +359,8 @@ extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int t
   a.out = static_cast<uint16_t*>(out);
   a.ldo = ldo;
   a.tokens = tokens;
+  a.m16 = 16;
+  a.m64 = 64;
   a.cols = cols;
   a.n_out = n_out;
   a.k_chunks = padded(cols, kChunkK) / kChunkK;

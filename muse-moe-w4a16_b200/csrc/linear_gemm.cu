@@ -2,14 +2,14 @@
 //
 // Swap-AB: 256 weight rows per pair are the MMA's M, up to 256 tokens its N, so a decode batch
 // wastes no rows of M. Per 128-code chunk a CTA copies its 128 rows' codes and scales (9 KiB, one
-// bulk copy each) into a six-deep ring; eight warps turn them into exact 16-bit weights in
+// bulk copy each) into a six-deep ring; sixteen warps turn them into exact 16-bit weights in
 // registers and write them as the K-major swizzled A operand (thread = weight row, one 128-byte
 // row of 64 k each); B is x by TMA, each CTA half of the tokens. Weights are dequantised once per
 // 256 tokens, which at ~140 instructions per thread and 64 k fits under the 512 clocks the MMAs
-// of a 256-token stage take. Accumulators are double buffered in tensor memory; the epilogue's
-// thread is a weight row, so for one token a warp stores 32 neighbouring outputs. A gated tile
-// holds 16 gate and the 16 matching up rows per warp: lanes i and i + 16 swap halves of a token
-// pair by one shuffle.
+// of a 256-token stage take. Accumulators are double buffered in tensor memory; the epilogue
+// reads them as matrix fragments and turns them over (rows are weight rows, y's rows are tokens)
+// with transposed matrix stores into shared memory, so that global stores run along y's rows. A
+// gated tile holds 16 gate rows and the 16 matching up rows per warp: one thread has both.
 // With fewer tiles than pairs K is split; a second kernel adds the fp32 partials in split order.
 // Bound by weight bytes and the dequantisation for tens of tokens, by the tensor pipe for hundreds.
 #undef MUSE_TRACE  // these kernels record no stamps
@@ -26,7 +26,8 @@ constexpr int kStageBytes = 2 * kABytes;
 constexpr int kCodes = 6;                    // code ring: 128-code chunks of 9 KiB
 constexpr int kCodeBytes = kTileCodeBytes + kTileScaleBytes;
 constexpr int kMaxBn = 256;
-constexpr int kDeqWarp0 = 4, kEpiWarp0 = 12, kThreads = 512;
+constexpr int kPatch = 32 * 64;              // an epilogue warp's outputs of 32 tokens, 64 bytes each
+constexpr int kDeqWarp0 = 4, kEpiWarp0 = 20, kThreads = 768;
 
 struct Ctl {
   uint64_t full[kStages], empty[kStages];
@@ -34,7 +35,7 @@ struct Ctl {
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem;
 };
-constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + (size_t)kCodes * kCodeBytes + sizeof(Ctl);
+constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + (size_t)kCodes * kCodeBytes + 4 * kPatch + sizeof(Ctl);
 static_assert(kSmem <= 232448, "shared memory of one CTA");
 
 struct GemmPlan {
@@ -46,6 +47,7 @@ struct Args {
   GemmPlan p;
   uint32_t idesc;
   uint32_t b_bytes;    // one CTA's B bytes per stage
+  int out_vec, add_vec;  // rows of out / add are 16-byte aligned
   float* partials;     // null: write the outputs
   int* error_flag;
 };
@@ -82,13 +84,46 @@ struct Pos {
   }
 };
 
+// 16-byte piece `p` of token row `tok` of a patch; pieces are swizzled so that eight token rows of
+// one piece, and the four pieces of two rows, lie in different banks.
+__device__ __forceinline__ uint32_t patch_row(const uint8_t* patch, int tok, int p) {
+  return ptx::smem_u32(patch) + tok * 64 + ((p ^ ((tok >> 1) & 3)) << 4);
+}
+// A patch of toks x outs 16-bit values to (kStore) or from rows tok0.. of a matrix.
+template <int kOut, bool kStore>
+__device__ __forceinline__ void copy_patch(uint8_t* patch, int lane, uint16_t* base, long long ld, int tok0, int toks,
+                                           int outs, int vec) {
+  constexpr int kPieces = kOut / 8;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int tok = i * (32 / kPieces) + lane / kPieces, p = lane % kPieces;
+    if (tok >= toks) continue;
+    uint8_t* at = patch + tok * 64 + ((p ^ ((tok >> 1) & 3)) << 4);
+    uint16_t* g = base + (size_t)(tok0 + tok) * ld + 8 * p;
+    if (vec && 8 * p + 8 <= outs) {
+      if (kStore)
+        *reinterpret_cast<uint4*>(g) = *reinterpret_cast<const uint4*>(at);
+      else
+        *reinterpret_cast<uint4*>(at) = __ldg(reinterpret_cast<const uint4*>(g));
+    } else {
+      for (int j = 0; j < 8 && 8 * p + j < outs; ++j) {
+        if (kStore)
+          g[j] = reinterpret_cast<const uint16_t*>(at)[j];
+        else
+          reinterpret_cast<uint16_t*>(at)[j] = __ldg(g + j);
+      }
+    }
+  }
+}
+
 template <bool kHalf, bool kGated>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* codes = smem + kStages * kStageBytes;
-  Ctl& ctl = *reinterpret_cast<Ctl*>(codes + kCodes * kCodeBytes);
+  uint8_t* patches = codes + kCodes * kCodeBytes;
+  Ctl& ctl = *reinterpret_cast<Ctl*>(patches + 4 * kPatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -202,14 +237,17 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
       }
     }
   } else if (warp >= kDeqWarp0 && warp < kEpiWarp0) {
-    const int h = (warp - kDeqWarp0) >> 2;            // 64-k half of the chunk
+    // four groups of four warps: group (p, h) takes half h of every second chunk
+    const int h = ((warp - kDeqWarp0) >> 2) & 1;      // 64-k half of the chunk
     const int r = (warp & 3) * 32 + lane;             // weight row of the tile
+    bool mine = warp < kDeqWarp0 + 8;
     Pos q, s;
     if (h) s.next(kStages);
     for (int w = pair; w < total && ok; w += pairs) {
       const Tile t = tile_of(a.p, k_chunks, w, rank);
-      for (int c = t.c0; c < t.c1; ++c) {
-        if (!ptx::mbar_wait_sleep(&ctl.code_full[q.slot], q.phase)) {
+      for (int c = t.c0; c < t.c1; ++c, mine = !mine, q.next(kCodes), s.next(kStages), s.next(kStages)) {
+        if (!mine) continue;
+        if (!warp_wait(&ctl.code_full[q.slot], q.phase)) {
           ok = false;
           break;
         }
@@ -222,7 +260,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
         uint32_t scale[4];
         expand_scales<kHalf>(sc & 0xFFFF, scale[0], scale[1]);
         expand_scales<kHalf>(sc >> 16, scale[2], scale[3]);
-        if (!ptx::mbar_wait_sleep(&ctl.empty[s.slot], s.phase ^ 1)) {
+        if (!warp_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
           ok = false;
           break;
         }
@@ -231,15 +269,12 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           uint32_t v[4];
-          dequant_word<kHalf>(word[i], scale[i >> 1], v);
+          dequant_word<kHalf>(word[i], scale[i >> 1], a.l.m16, a.l.m64, v);
           *reinterpret_cast<uint4*>(dst + ((i ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], 0));
-        q.next(kCodes);
-        s.next(kStages);
-        s.next(kStages);
       }
     }
   } else if (warp >= kEpiWarp0) {
@@ -248,11 +283,12 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
     const uint32_t lane_base = tmem + ((uint32_t)quarter << 21);
     constexpr int dtype = kHalf ? kFp16 : kBf16;
     const float gs = __ldg(a.l.gs) * kUnscale<kHalf>;
+    uint8_t* patch = patches + (warp - kEpiWarp0) * kPatch;
     int it = 0;
     for (int w = pair; w < total; w += pairs, ++it) {
       const Tile t = tile_of(a.p, k_chunks, w, rank);
       const int buf = it & 1;
-      if (!ptx::mbar_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
+      if (!warp_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
         ok = false;
         break;
       }
@@ -262,38 +298,67 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
       const bool tile_ok = t.m_tile * kTileM < a.l.padded_rows;
       const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
       for (int c = 0; c < n_tok && tile_ok; c += 32) {
-        float v[32];
-        tmem_ld32(acc + c, v);
-        ptx::tmem_wait_ld();
         if (a.partials) {
+          float v[32];
+          tmem_ld32(acc + c, v);
+          ptx::tmem_wait_ld();
           float* to = a.partials + ((size_t)t.split * a.l.tokens + t.tok0 + c) * a.l.padded_rows + row;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             if (c + j < n_tok) to[(size_t)j * a.l.padded_rows] = v[j];
-        } else if (kGated) {
-          // lanes 0-15 take the even token of a pair, 16-31 the odd one
-          const bool upper = lane & 16;
-          const int o = t.m_tile * 64 + quarter * 16 + (lane & 15);
+          continue;
+        }
+        // fragments of rows 0-15 and 16-31 of the warp's quarter (gated: gate and up of the same
+        // outputs), through a transposed patch [token][output] so that stores run along outputs
+        float lo[16], hi[16];
+        tmem_ld_frag(acc + c, lo);
+        tmem_ld_frag(acc + c + (16u << 16), hi);
+        ptx::tmem_wait_ld();
+        constexpr int kOut = kGated ? 16 : 32;              // outputs of the warp
+        const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
+        const int tok0 = t.tok0 + c, toks = min(32, n_tok - c), outs = min(kOut, a.l.n_out - o0);
+        __syncwarp();                                       // the patch's last readers are done
+        if (outs > 0 && a.l.add) {
+          copy_patch<kOut, false>(patch, lane, const_cast<uint16_t*>(a.l.add) + o0, a.l.ld_add, tok0, toks, outs, a.add_vec);
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float other = __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j + 1], 16);
-            const float gate = (upper ? other : v[j]) * gs, up = (upper ? v[j + 1] : other) * gs;
-            const int tok = c + j + (upper ? 1 : 0);
-            if (tok < n_tok && o < a.l.n_out) {
-              float y = silu_f(gate) * up;
-              if (a.l.add) y += load16(dtype, a.l.add + (size_t)(t.tok0 + tok) * a.l.ld_add + o);
-              a.l.out[(size_t)(t.tok0 + tok) * a.l.ldo + o] = round16(dtype, y);
+          for (int b = 0; b < 4; ++b) {
+            uint32_t f[kGated ? 2 : 4];
+            ldmatrix2_t(patch_row(patch, 8 * b + (lane & 7), (lane >> 3) & 1), f[0], f[1]);
+            if (!kGated) ldmatrix2_t(patch_row(patch, 8 * b + (lane & 7), 2 + ((lane >> 3) & 1)), f[2], f[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 u = unpack16(dtype, f[i]);
+              if (kGated) {
+                lo[4 * b + 2 * i] = silu_f(lo[4 * b + 2 * i] * gs) * (hi[4 * b + 2 * i] * gs) + u.x;
+                lo[4 * b + 2 * i + 1] = silu_f(lo[4 * b + 2 * i + 1] * gs) * (hi[4 * b + 2 * i + 1] * gs) + u.y;
+              } else {
+                const float2 w2 = unpack16(dtype, f[2 + i]);
+                lo[4 * b + 2 * i] = lo[4 * b + 2 * i] * gs + u.x;
+                lo[4 * b + 2 * i + 1] = lo[4 * b + 2 * i + 1] * gs + u.y;
+                hi[4 * b + 2 * i] = hi[4 * b + 2 * i] * gs + w2.x;
+                hi[4 * b + 2 * i + 1] = hi[4 * b + 2 * i + 1] * gs + w2.y;
+              }
             }
           }
-        } else if (row < a.l.n_out) {
+          __syncwarp();
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < n_tok) {
-              float y = v[j] * gs;
-              if (a.l.add) y += load16(dtype, a.l.add + (size_t)(t.tok0 + c + j) * a.l.ld_add + row);
-              a.l.out[(size_t)(t.tok0 + c + j) * a.l.ldo + row] = round16(dtype, y);
-            }
+          for (int j = 0; j < 16; ++j) {
+            lo[j] = kGated ? silu_f(lo[j] * gs) * (hi[j] * gs) : lo[j] * gs;
+            hi[j] *= gs;
+          }
         }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          stmatrix2_t(patch_row(patch, 8 * b + (lane & 7), (lane >> 3) & 1), pack16(dtype, lo[4 * b], lo[4 * b + 1]),
+                      pack16(dtype, lo[4 * b + 2], lo[4 * b + 3]));
+          if (!kGated)
+            stmatrix2_t(patch_row(patch, 8 * b + (lane & 7), 2 + ((lane >> 3) & 1)),
+                        pack16(dtype, hi[4 * b], hi[4 * b + 1]), pack16(dtype, hi[4 * b + 2], hi[4 * b + 3]));
+        }
+        __syncwarp();
+        if (outs > 0) copy_patch<kOut, true>(patch, lane, a.l.out + o0, a.l.ldo, tok0, toks, outs, a.out_vec);
       }
       ptx::tc_fence_before();
       __syncwarp();
@@ -404,6 +469,9 @@ int launch_linear_gemm(const LinearArgs& l, int dtype, bool gated, float* partia
   const uint32_t type = dtype == kBf16 ? 1u : 0u;
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(a.p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
   a.b_bytes = (uint32_t)a.p.bn / 2 * 128;
+  auto vec = [](const void* p, long long ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
+  a.out_vec = vec(l.out, l.ldo);
+  a.add_vec = vec(l.add, l.ld_add);
   a.partials = a.p.splits > 1 ? partials : nullptr;
   a.error_flag = error_flag;
   CUtensorMap map;

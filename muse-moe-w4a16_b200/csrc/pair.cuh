@@ -22,8 +22,11 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(ptx::smem_u32(p)), "r"(rank));
   return r;
 }
+// Arrive on a barrier of either CTA. What it announces is ordered by the fence that precedes it
+// (fence.proxy.async for operands in shared memory, tcgen05.fence for tensor memory reads); a
+// release at cluster scope would also wait ~1300 clocks for this thread's earlier stores.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // TMA box into this CTA's shared memory, completing on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
@@ -60,6 +63,26 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
       : "r"(taddr));
 }
 
+// 16 accumulator rows (tensor-memory lanes) x 32 columns, as the fragments of four 16 x 8 blocks:
+// v[4 b + i] is row lane / 4 + 8 (i / 2), column 8 b + 2 (lane % 4) + i % 2.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// Two 8 x 8 blocks of 16-bit pairs (fragments as above) to and from shared memory, transposed: the
+// address of lane l (l < 16) is the 16-byte row that holds column l % 8 of block l / 8.
+__device__ __forceinline__ void stmatrix2_t(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void ldmatrix2_t(uint32_t addr, uint32_t& a, uint32_t& b) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
+}
+
 // Shared-memory descriptors, 128-byte swizzle. K-major: rows of 64 k, 8-row groups 1024 B apart.
 // MN-major: boxes of 64 (m or n) x 64 k, 8192 B apart (the leading offset); 8-k groups 1024 B
 // apart (the stride offset).
@@ -75,6 +98,19 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
 // Descriptor step of 16 k (in 16-byte units).
 template <bool kMn>
 constexpr uint32_t kStepDesc = kMn ? 16 * 128 / 16 : 2;
+
+// A whole warp waits for a phase: one lane polls (every polling lane is an access of its own to the
+// barrier, and the others' would slow the arrivals), the rest wait for it.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait(bar, parity);
+  return __shfl_sync(0xffffffffu, ok, 0);
+}
+__device__ __forceinline__ bool warp_wait_sleep(uint64_t* bar, uint32_t parity) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait_sleep(bar, parity);
+  return __shfl_sync(0xffffffffu, ok, 0);
+}
 
 // After an expired wait: report it, and leave copies and MMAs in flight time to land before the
 // shared and tensor memory go.

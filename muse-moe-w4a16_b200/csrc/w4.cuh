@@ -22,6 +22,7 @@ struct LinearArgs {
   int k_chunks;              // 128-code chunks of K
   int padded_rows;           // weight rows, padded to 128
   int tile_tokens;           // few tokens: tokens per CTA (x staging rows)
+  uint32_t m16, m64;         // 16 and 64 (see dequant_word)
 };
 
 // The product for more than a few tokens (linear_gemm.cu).
@@ -59,13 +60,14 @@ __device__ __forceinline__ void expand_scales(uint32_t two, uint32_t& s0, uint32
 
 // One permuted code word -> four pairs (natural element order) times the scale register.
 // The masked bits read as bf16 are e2m1 * 2^-126; with the scale the result is e2m1 * e4m3 * 2^-8,
-// six significant bits: exact. For fp16 the three magnitude bits move up by three (e2m1 * 2^-14);
+// six significant bits: exact. The logic pipe is the busiest one here, so two of the shifts are
+// multiplies by m16 = 16 and m64 = 64, which the compiler cannot see. For fp16 the three magnitude bits move up by three (e2m1 * 2^-14);
 // times s * 2^5, then times 2^9: e2m1 * e4m3, exact (every step is a multiple of 2^-24).
 template <bool kHalf>
-__device__ __forceinline__ void dequant_word(uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
+__device__ __forceinline__ void dequant_word(uint32_t w, uint32_t scale, uint32_t m16, uint32_t m64, uint32_t (&out)[4]) {
   constexpr uint32_t kMask = 0x81C081C0u;
-  uint32_t v[4] = {w & kMask, ptx::rotl(w, 4) & kMask, ptx::rotl(w, 10) & kMask,
-                   ((w << 6) & 0x80C080C0u) | ((w >> 2) & 0x01000100u)};
+  uint32_t v[4] = {w & kMask, (w * m16) & kMask, ptx::rotl(w, 10) & kMask,
+                   ((w * m64) & 0x80C080C0u) | ((w >> 2) & 0x01000100u)};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (kHalf) {
