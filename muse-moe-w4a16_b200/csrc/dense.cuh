@@ -57,7 +57,10 @@ int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k,
 
 // ---- 16-bit conversions shared by the dense kernels
 
-__device__ __forceinline__ float silu_f(float a) { return a / (1.f + __expf(-a)); }
+// Logistic function and silu with the fast division (2 steps of 2^-24; its range ends at 2^126, where
+// the result is below 2^-118 and becomes 0): the exact one's slow path is a branch per element.
+__device__ __forceinline__ float sigmoid_f(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
+__device__ __forceinline__ float silu_f(float a) { return __fdividef(a, 1.f + __expf(-a)); }
 
 __device__ __forceinline__ uint32_t pack16(int dtype, float lo, float hi) {
   uint32_t r;

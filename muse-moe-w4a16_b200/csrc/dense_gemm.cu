@@ -99,7 +99,7 @@ __device__ __forceinline__ float4 add4(int dtype, const void* base, long long ld
 // da, db and h of four elements from dh, a, b:  s = 1 / (1 + exp(-a)),
 // da = dh * b * s * (1 + a * (1 - s)), db = dh * a * s, h = a * s * b.
 __device__ __forceinline__ void dgate1(float dh, float a, float b, float& da, float& db, float& h) {
-  const float s = 1.f / (1.f + __expf(-a));
+  const float s = sigmoid_f(a);
   const float as = a * s;
   da = dh * b * (s + as * (1.f - s));
   db = dh * as;

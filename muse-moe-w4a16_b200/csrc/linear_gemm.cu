@@ -20,9 +20,9 @@
 namespace muse {
 namespace {
 
-constexpr int kStages = 5;                   // 64-k stages: A (16 KiB) and half of B (16 KiB)
+constexpr int kMaxStages = 9;
 constexpr int kABytes = kTileM * 128;
-constexpr int kStageBytes = 2 * kABytes;
+constexpr int kRingBytes = 5 * 2 * kABytes;  // 64-k stages: A (16 KiB) and half of B (64 bytes a token)
 constexpr int kCodes = 6;                    // code ring: 128-code chunks of 9 KiB
 constexpr int kCodeBytes = kTileCodeBytes + kTileScaleBytes;
 constexpr int kMaxBn = 256;
@@ -30,16 +30,16 @@ constexpr int kPatch = 32 * 64;              // an epilogue warp's outputs of 32
 constexpr int kDeqWarp0 = 4, kEpiWarp0 = 20, kThreads = 768;
 
 struct Ctl {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t code_full[kCodes], code_empty[kCodes];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem;
 };
-constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + (size_t)kCodes * kCodeBytes + 4 * kPatch + sizeof(Ctl);
+constexpr size_t kSmem = 1024 + (size_t)kRingBytes + (size_t)kCodes * kCodeBytes + 4 * kPatch + sizeof(Ctl);
 static_assert(kSmem <= 232448, "shared memory of one CTA");
 
 struct GemmPlan {
-  int bn, tiles_m, tiles_n, splits, chunks_per_split;
+  int bn, stages, tiles_m, tiles_n, splits, chunks_per_split;
 };
 
 struct Args {
@@ -89,39 +89,64 @@ struct Pos {
 __device__ __forceinline__ uint32_t patch_row(const uint8_t* patch, int tok, int p) {
   return ptx::smem_u32(patch) + tok * 64 + ((p ^ ((tok >> 1) & 3)) << 4);
 }
-// A patch of toks x outs 16-bit values to (kStore) or from rows tok0.. of a matrix.
-template <int kOut, bool kStore>
-__device__ __forceinline__ void copy_patch(uint8_t* patch, int lane, uint16_t* base, long long ld, int tok0, int toks,
-                                           int outs, int vec) {
-  constexpr int kPieces = kOut / 8;
+// A patch of up to 32 tokens x outs 16-bit values: lane pieces (token, piece) of it.
+template <int kOut>
+struct PatchIo {
+  static constexpr int kPieces = kOut / 8;
+  // from rows tok0.. of a matrix into registers (all loads in flight together)
+  static __device__ __forceinline__ void load(uint4 (&v)[kPieces], int lane, const uint16_t* base, long long ld, int tok0,
+                                              int toks, int outs, int vec) {
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int tok = i * (32 / kPieces) + lane / kPieces, p = lane % kPieces;
-    if (tok >= toks) continue;
-    uint8_t* at = patch + tok * 64 + ((p ^ ((tok >> 1) & 3)) << 4);
-    uint16_t* g = base + (size_t)(tok0 + tok) * ld + 8 * p;
-    if (vec && 8 * p + 8 <= outs) {
-      if (kStore)
-        *reinterpret_cast<uint4*>(g) = *reinterpret_cast<const uint4*>(at);
-      else
-        *reinterpret_cast<uint4*>(at) = __ldg(reinterpret_cast<const uint4*>(g));
-    } else {
-      for (int j = 0; j < 8 && 8 * p + j < outs; ++j) {
-        if (kStore)
-          g[j] = reinterpret_cast<const uint16_t*>(at)[j];
-        else
-          reinterpret_cast<uint16_t*>(at)[j] = __ldg(g + j);
+    for (int i = 0; i < kPieces; ++i) {
+      const int tok = i * (32 / kPieces) + lane / kPieces, p = lane % kPieces;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (tok >= toks) continue;
+      const uint16_t* g = base + (size_t)(tok0 + tok) * ld + 8 * p;
+      if (vec && 8 * p + 8 <= outs) {
+        v[i] = __ldg(reinterpret_cast<const uint4*>(g));
+      } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = 8 * p + j < outs ? __ldg(g + j) : 0;
+        v[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
       }
     }
   }
-}
+  static __device__ __forceinline__ void put(uint8_t* patch, int lane, const uint4 (&v)[kPieces]) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int tok = i * (32 / kPieces) + lane / kPieces, p = lane % kPieces;
+      *reinterpret_cast<uint4*>(patch + tok * 64 + ((p ^ ((tok >> 1) & 3)) << 4)) = v[i];
+    }
+  }
+  // from the patch to rows tok0.. of a matrix
+  static __device__ __forceinline__ void store(const uint8_t* patch, int lane, uint16_t* base, long long ld, int tok0,
+                                               int toks, int outs, int vec) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int tok = i * (32 / kPieces) + lane / kPieces, p = lane % kPieces;
+      if (tok >= toks) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(patch + tok * 64 + ((p ^ ((tok >> 1) & 3)) << 4));
+      uint16_t* g = base + (size_t)(tok0 + tok) * ld + 8 * p;
+      if (vec && 8 * p + 8 <= outs) {
+        *reinterpret_cast<uint4*>(g) = v;
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (8 * p + j < outs) g[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+  }
+};
 
 template <bool kHalf, bool kGated>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* codes = smem + kStages * kStageBytes;
+  uint8_t* codes = smem + kRingBytes;
+  const int n_stages = a.p.stages, stage_bytes = kABytes + a.p.bn * 64;
   uint8_t* patches = codes + kCodes * kCodeBytes;
   Ctl& ctl = *reinterpret_cast<Ctl*>(patches + 4 * kPatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -131,7 +156,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
   const int k_chunks = a.l.k_chunks;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < n_stages; ++s) {
       ptx::mbar_init(&ctl.full[s], 1 + 2 * 4);  // B bytes announced by the leader; A by four warps of each CTA
       ptx::mbar_init(&ctl.empty[s], 1);
     }
@@ -201,13 +226,13 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t sa = ptx::smem_u32(smem + s.slot * kStageBytes);
+          const uint32_t sa = ptx::smem_u32(smem + s.slot * stage_bytes);
           const uint64_t da = operand_desc<false>(sa), db = operand_desc<false>(sa + kABytes);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, n > 2 * t.c0 || j > 0);
           commit_pair(&ctl.empty[s.slot]);
-          s.next(kStages);
+          s.next(n_stages);
         }
         commit_pair(&ctl.acc_full[buf]);
       }
@@ -225,15 +250,15 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
             break;
           }
           if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], 2 * a.b_bytes);
-          tma_pair(ptx::smem_u32(smem + s.slot * kStageBytes) + kABytes, &map_x, n * 64, row,
+          tma_pair(ptx::smem_u32(smem + s.slot * stage_bytes) + kABytes, &map_x, n * 64, row,
                    map_rank(&ctl.full[s.slot], 0));
-          s.next(kStages);
+          s.next(n_stages);
         }
       }
       // the commits that free the last stages arrive here too: see them land before leaving
-      for (int i = 0; i < kStages && ok; ++i) {
+      for (int i = 0; i < n_stages && ok; ++i) {
         if (!ptx::mbar_wait(&ctl.empty[s.slot], s.phase ^ 1)) ok = false;
-        s.next(kStages);
+        s.next(n_stages);
       }
     }
   } else if (warp >= kDeqWarp0 && warp < kEpiWarp0) {
@@ -242,10 +267,10 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
     const int r = (warp & 3) * 32 + lane;             // weight row of the tile
     bool mine = warp < kDeqWarp0 + 8;
     Pos q, s;
-    if (h) s.next(kStages);
+    if (h) s.next(n_stages);
     for (int w = pair; w < total && ok; w += pairs) {
       const Tile t = tile_of(a.p, k_chunks, w, rank);
-      for (int c = t.c0; c < t.c1; ++c, mine = !mine, q.next(kCodes), s.next(kStages), s.next(kStages)) {
+      for (int c = t.c0; c < t.c1; ++c, mine = !mine, q.next(kCodes), s.next(n_stages), s.next(n_stages)) {
         if (!mine) continue;
         if (!warp_wait(&ctl.code_full[q.slot], q.phase)) {
           ok = false;
@@ -264,7 +289,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
           ok = false;
           break;
         }
-        uint8_t* dst = smem + s.slot * kStageBytes + r * 128;
+        uint8_t* dst = smem + s.slot * stage_bytes + r * 128;
         const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -288,6 +313,14 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
     for (int w = pair; w < total; w += pairs, ++it) {
       const Tile t = tile_of(a.p, k_chunks, w, rank);
       const int buf = it & 1;
+      constexpr int kOut = kGated ? 16 : 32;              // outputs of the warp
+      using Io = PatchIo<kOut>;
+      const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
+      const int outs = min(kOut, a.l.n_out - o0);
+      const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
+      const bool adds = a.l.add && !a.partials && outs > 0;
+      uint4 ahead[Io::kPieces];                           // the next patch's addend
+      if (adds) Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, t.tok0, min(32, n_tok), outs, a.add_vec);
       if (!warp_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
         ok = false;
         break;
@@ -296,7 +329,6 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
       const uint32_t acc = lane_base + buf * kMaxBn;
       const int row = t.m_tile * kTileM + quarter * 32 + lane;   // padded weight row
       const bool tile_ok = t.m_tile * kTileM < a.l.padded_rows;
-      const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
       for (int c = 0; c < n_tok && tile_ok; c += 32) {
         if (a.partials) {
           float v[32];
@@ -314,12 +346,12 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
         tmem_ld_frag(acc + c, lo);
         tmem_ld_frag(acc + c + (16u << 16), hi);
         ptx::tmem_wait_ld();
-        constexpr int kOut = kGated ? 16 : 32;              // outputs of the warp
-        const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
-        const int tok0 = t.tok0 + c, toks = min(32, n_tok - c), outs = min(kOut, a.l.n_out - o0);
+        const int tok0 = t.tok0 + c, toks = min(32, n_tok - c);
         __syncwarp();                                       // the patch's last readers are done
-        if (outs > 0 && a.l.add) {
-          copy_patch<kOut, false>(patch, lane, const_cast<uint16_t*>(a.l.add) + o0, a.l.ld_add, tok0, toks, outs, a.add_vec);
+        if (adds) {
+          Io::put(patch, lane, ahead);
+          if (c + 32 < n_tok)
+            Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, tok0 + 32, min(32, n_tok - c - 32), outs, a.add_vec);
           __syncwarp();
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
@@ -358,7 +390,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
                         pack16(dtype, hi[4 * b], hi[4 * b + 1]), pack16(dtype, hi[4 * b + 2], hi[4 * b + 3]));
         }
         __syncwarp();
-        if (outs > 0) copy_patch<kOut, true>(patch, lane, a.l.out + o0, a.l.ldo, tok0, toks, outs, a.out_vec);
+        if (outs > 0) Io::store(patch, lane, a.l.out + o0, a.l.ldo, tok0, toks, outs, a.out_vec);
       }
       ptx::tc_fence_before();
       __syncwarp();
@@ -404,8 +436,8 @@ __global__ void __launch_bounds__(256) linear_reduce(const Args a) {
 constexpr int kPairs = 74;  // 148 SMs, two to a pair
 
 // Token tile and split of K from the sizes alone: the least estimated time in SM clocks. A 64-k
-// stage costs the most of its MMAs (2 bn), its B rows from L2 (~60 B per clock) and the
-// dequantisation (~190); a tile's start and epilogue 2000 + 8 per token; a split the second
+// stage costs its MMAs (2 bn) or the ring's latency over its depth (~2600 from a freed stage over
+// dequantisation, cluster arrival, MMA and commit to the next free one); a tile's start and epilogue 2000 + 8 per token; a split the second
 // kernel's launch and the partials' way through L2 (~2 KB per clock over the chip).
 GemmPlan make_plan(int tokens, int padded_rows, int k_chunks) {
   GemmPlan best{};
@@ -416,9 +448,10 @@ GemmPlan make_plan(int tokens, int padded_rows, int k_chunks) {
     p.tiles_m = (padded_rows + 255) / 256;
     p.tiles_n = (tokens + bn - 1) / bn;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    double stage = 190;
+    p.stages = kRingBytes / (kABytes + bn * 64);
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    double stage = 2600.0 / p.stages;
     if (2.0 * bn > stage) stage = 2.0 * bn;
-    if (bn * 64 / 60.0 > stage) stage = bn * 64 / 60.0;
     for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= kPairs && k_chunks / s >= 2)); ++s) {
       p.chunks_per_split = (k_chunks + s - 1) / s;
       p.splits = (k_chunks + p.chunks_per_split - 1) / p.chunks_per_split;
