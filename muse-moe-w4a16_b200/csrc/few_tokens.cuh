@@ -1,0 +1,31 @@
+// Launch interface of the few-token products (few_tokens.cu).
+#pragma once
+
+#include "w4.cuh"
+
+namespace muse {
+
+// The most tokens of a few-token call.
+constexpr int kFewTokens = 32;
+
+struct FewArgs {
+  const uint8_t* wq;      // NVFP4: prepared codes, scales and the global scale
+  const uint8_t* wsf;
+  const float* gs;
+  const uint16_t* add;
+  long long ld_add;
+  uint16_t* out;
+  long long ldo;
+  float* ab;              // gated 16-bit weights: pre-activations to keep, or null
+  int tokens, n_out, up_row;
+  int stages;             // stages of K: 128 codes or 64 16-bit columns
+  int ranks, stages_per_rank, depth;  // set by the launch
+  uint32_t m16, m64;
+  int* error_flag;
+};
+
+int launch_few_w4(const LinearArgs& l, int dtype, bool gated, int* error_flag, cudaStream_t st);
+// A forward product of the feed-forward block (modes kStore and kGate, both operands along k).
+int launch_few_dense(const DenseGemm& g, cudaStream_t st);
+
+}  // namespace muse

@@ -8,7 +8,7 @@
 // operands of dx and dW13), each once from fp32. The pre-activations are kept in fp32 for the
 // backward pass, 8 T I bytes: kept in 16 bits their rounding would enter da, db and h a second
 // time. h is recomputed from them, to the same bits, rather than kept.
-#include "dense.cuh"
+#include "few_tokens.cuh"
 #include "kernels.cuh"
 
 namespace muse {
@@ -39,8 +39,8 @@ FfnLayout ffn_layout(int t, int hidden, int inter, bool backward) {
                 most(dense_scratch_bytes(2 * inter, hidden, t, kStore, false),
                      dense_scratch_bytes(hidden, inter, t, kStore, false)));
   else
-    part = most(dense_scratch_bytes(t, 2 * inter, hidden, kGate, true),
-                dense_scratch_bytes(t, hidden, inter, kStore, true));
+    part = t <= kFewTokens ? 0 : most(dense_scratch_bytes(t, 2 * inter, hidden, kGate, true),
+                                      dense_scratch_bytes(t, hidden, inter, kStore, true));
   l.h = 0;
   l.dab = up((size_t)2 * t * inter);
   l.partials = l.dab + (backward ? up((size_t)4 * t * inter) : 0);
@@ -92,7 +92,9 @@ extern "C" int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int
   g.mode = kGate;
   g.out = ws + l.h, g.ldo = inter;
   g.ab = ab;
-  if ((rc = launch_dense_gemm(g, (cudaStream_t)stream))) return rc;
+  // up to kFewTokens tokens the weights are streamed, beyond the tensor-core pairs take over
+  const auto product = tokens <= kFewTokens ? launch_few_dense : launch_dense_gemm;
+  if ((rc = product(g, (cudaStream_t)stream))) return rc;
   g.a = {ws + l.h, inter, true};
   g.b = {w2, ld2, true};
   g.n = hidden, g.k = inter;
@@ -100,7 +102,7 @@ extern "C" int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int
   g.out = out, g.ldo = hidden;
   g.ab = nullptr;
   g.add = add, g.ld_add = ld_add;
-  return launch_dense_gemm(g, (cudaStream_t)stream);
+  return product(g, (cudaStream_t)stream);
 }
 
 extern "C" int muse_moe_ffn_backward(const void* dy, long long ldy, const void* x, long long ldx, int dtype, int tokens,

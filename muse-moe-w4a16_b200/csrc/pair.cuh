@@ -104,12 +104,16 @@ constexpr uint32_t kStepDesc = kMn ? 16 * 128 / 16 : 2;
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   int ok = 1;
   if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait(bar, parity);
-  return __shfl_sync(0xffffffffu, ok, 0);
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();  // orders the other lanes' reads after the phase
+  return ok;
 }
 __device__ __forceinline__ bool warp_wait_sleep(uint64_t* bar, uint32_t parity) {
   int ok = 1;
   if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait_sleep(bar, parity);
-  return __shfl_sync(0xffffffffu, ok, 0);
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();  // orders the other lanes' reads after the phase
+  return ok;
 }
 
 // After an expired wait: report it, and leave copies and MMAs in flight time to land before the

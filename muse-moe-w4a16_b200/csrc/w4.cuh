@@ -1,5 +1,5 @@
 // In-register dequantisation of prepared NVFP4 code words (layout.cuh) and the launch interface
-// between the two dense 4-bit kernels (linear.cu, linear_gemm.cu).
+// of the many-token 4-bit product (linear_gemm.cu).
 #pragma once
 
 #include "dense.cuh"
@@ -21,11 +21,10 @@ struct LinearArgs {
   int tokens, cols, n_out;   // n_out: columns of y
   int k_chunks;              // 128-code chunks of K
   int padded_rows;           // weight rows, padded to 128
-  int tile_tokens;           // few tokens: tokens per CTA (x staging rows)
   uint32_t m16, m64;         // 16 and 64 (see dequant_word)
 };
 
-// The product for more than a few tokens (linear_gemm.cu).
+// The product for more than a few tokens.
 size_t linear_gemm_scratch_bytes(int tokens, int padded_rows, int k_chunks);
 int launch_linear_gemm(const LinearArgs& a, int dtype, bool gated, float* partials, int* error_flag, cudaStream_t st);
 
