@@ -371,14 +371,14 @@ int muse_moe_forward_noalloc(const void* x, const int32_t* topk_ids, const float
  * 16-bit weights; ld* are row strides in elements. out may not overlap an input.
  *
  * muse_moe_linear_prepared_size / muse_moe_prepare_linear: a row-major NVFP4 matrix w u8 [rows,
- * cols/2], w_sf e4m3 [rows, cols/16] in the experts' tile order (any rows; cols a multiple of 16;
- * rows and columns padded to 128 with zero codes). gated: rows [0, rows/2) are gate rows, the
+ * cols/2], w_sf e4m3 [rows, cols/16] in the experts' tile order, each tile's scales behind its codes
+ * (any rows; cols a multiple of 16; rows and columns padded to 128 with zero codes). gated: rows [0, rows/2) are gate rows, the
  * rest the matching up rows. No counterpart in the reference, whose prepare (baseline.py:82-103)
  * repacks routed experts only.
  */
-int muse_moe_linear_prepared_size(int rows, int cols, int gated, size_t* code_bytes, size_t* scale_bytes);
-int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int cols, int gated,
-                            uint8_t* w_out, uint8_t* w_sf_out, muse_stream_t stream);
+int muse_moe_linear_prepared_size(int rows, int cols, int gated, size_t* bytes);
+int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int cols, int gated, uint8_t* out,
+                            muse_stream_t stream);
 
 /*
  * out[t, n] = gs * sum_k x[t, k] * e2m1[n, k] * e4m3[n, k/16] (+ add[t, n]), or with gated
@@ -389,8 +389,7 @@ int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int
  */
 int muse_moe_linear_workspace_size(int tokens, int rows, int cols, int gated, size_t* bytes);
 int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int rows, int cols, int gated,
-                       const uint8_t* wp, const uint8_t* w_sfp, const float* w_gs, const void* add,
-                       long long ld_add, void* out, long long ldo, void* workspace, size_t workspace_bytes,
+                       const uint8_t* wp, const float* w_gs, const void* add, long long ld_add, void* out, long long ldo, void* workspace, size_t workspace_bytes,
                        muse_stream_t stream);
 
 /*

@@ -2,14 +2,15 @@
 // prepared NVFP4 tiles or 16-bit rows.
 //
 // A CTA takes 128 weight rows (gated 16-bit weights: 64 gate rows and the 64 matching up rows) and a
-// cluster of CTAs splits K. One thread copies whole stages into a ring of shared memory -- NVFP4:
-// the 9 KiB tile of 128 k by two bulk copies; 16 bits: 64 k by TMA -- together with the tokens'
-// columns (TMA, rows past the last token read as zeros). Each of eight warps multiplies its
-// own 16 rows by mma.sync m16n8k16: tokens are the 8-wide side, so one token wastes no weight
-// traffic, and at 32 tokens the matrix pipe still keeps up with HBM. Lanes read operands as 16-byte
-// pieces along k: the order of k inside a stage is the lanes', the same for both operands, so no
-// shuffle is needed. There is no reduction inside a CTA; the ranks' sums meet once, in rank order,
-// through distributed shared memory, each rank finishing its share of the rows.
+// cluster of CTAs splits K. One thread copies the weights into a ring of shared memory, 128 codes
+// or 64 16-bit columns to a stage (one bulk copy of a tile, or a TMA box), and the same columns of
+// x (TMA; rows past the last token read as zeros). Eight warps multiply 16 rows each by mma.sync
+// m16n8k16: tokens are the 8-wide side, so one token wastes no weight traffic, and at 32 tokens the
+// matrix pipe still keeps up with HBM. Lanes read both operands as 16-byte pieces along k -- the order of k inside a
+// stage is the lanes' -- so nothing is shuffled. A CTA pushes its sums to the ranks that own the
+// outputs (16-byte stores to distributed shared memory, one cluster barrier), which add them in
+// rank order. Sixteen warps with half of a stage each measured slower (13.0 against 8.7 us at 1 x 7168 x
+// 4096 gated): for NVFP4 the instructions per code are what keeps the stream from HBM's rate.
 // Bound by the weights' bytes; the smallest sizes by launch, first-byte and cluster latency.
 #undef MUSE_TRACE  // these kernels record no stamps
 #include "few_tokens.cuh"
@@ -29,8 +30,10 @@ struct Ctl {
   uint64_t full[kMaxDepth], empty[kMaxDepth];
 };
 
+// A stage is 128 codes or 64 16-bit columns of the tile's rows.
 template <bool kW4> constexpr int kStageK = kW4 ? kChunkK : 64;
-template <bool kW4> constexpr int kWeightBytes = kW4 ? kTileCodeBytes + kTileScaleBytes : kTileM * 128;
+template <bool kW4> constexpr int kWeightBytes = kW4 ? kLinearTileBytes : kTileM * 128;
+// x: boxes of 64 columns x 8 kNT tokens.
 template <bool kW4, int kNT> constexpr int kStageBytes = kWeightBytes<kW4> + (kW4 ? 2 : 1) * kNT * 1024;
 
 // mma.sync m16n8k16, fp32 accumulators: 16 weight rows x 8 tokens x 16 k.
@@ -65,102 +68,116 @@ __global__ void __launch_bounds__(kThreads)
 few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const FewArgs a) {
   constexpr int kK = kStageK<kW4>, kWBytes = kWeightBytes<kW4>, kStage = kStageBytes<kW4, kNT>;
   constexpr int dtype = kHalf ? kFp16 : kBf16;
+  constexpr int kOut = kGated ? kTileM / 2 : kTileM;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + a.depth * kStage);
-  float* sums = reinterpret_cast<float*>(&ctl + 1);   // [token][kPitch]
+  const int toks = a.tokens, ranks = a.ranks;
+  float* recv = reinterpret_cast<float*>(smem + a.depth * kStage);  // [rank][token][128 / ranks]
+  float* sums = recv + toks * kTileM;                 // [token][kPitch], rows in the order of their owners
+  Ctl& ctl = *reinterpret_cast<Ctl*>(sums + toks * kPitch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_rank(), ranks = a.ranks;
+  const int rank = (int)cluster_rank();
   const int m_tile = blockIdx.x / ranks;
   const int first = rank * a.stages_per_rank;
-  const int n_stages = min(a.stages_per_rank, a.stages - first);   // may be <= 0 for a last rank
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < a.depth; ++s) {
-      ptx::mbar_init(&ctl.full[s], 1);
-      ptx::mbar_init(&ctl.empty[s], kWarps);
-    }
-    ptx::fence_barrier_init();
-  }
-  __syncthreads();
-  chain_release();
-
-  bool ok = true;
-  float acc[kNT][4];
-#pragma unroll
-  for (int n = 0; n < kNT; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+  const int n_stages = max(0, min(a.stages_per_rank, a.stages - first));
 
   if (warp == kWarps) {
-    if (ptx::elect_one()) {
-      auto load_w = [&](int i, uint64_t* bar) {
-        uint8_t* dst = smem + (i % a.depth) * kStage;
-        if (kW4) {
-          const size_t tile = (size_t)m_tile * a.stages + first + i;
-          ptx::bulk_g2s(dst, a.wq + tile * kTileCodeBytes, kTileCodeBytes, bar);
-          ptx::bulk_g2s(dst + kTileCodeBytes, a.wsf + tile * kTileScaleBytes, kTileScaleBytes, bar);
-        } else if (kGated) {
-          ptx::tma_load_2d(dst, &map_w, (first + i) * kK, m_tile * 64, bar);
-          ptx::tma_load_2d(dst + kWBytes / 2, &map_w, (first + i) * kK, a.up_row + m_tile * 64, bar);
-        } else {
-          ptx::tma_load_2d(dst, &map_w, (first + i) * kK, m_tile * kTileM, bar);
-        }
-      };
-      auto load_x = [&](int i, uint64_t* bar) {
-        uint8_t* dst = smem + (i % a.depth) * kStage + kWBytes;
-        ptx::tma_load_2d(dst, &map_x, (first + i) * kK, 0, bar);
-        if (kW4) ptx::tma_load_2d(dst + kNT * 1024, &map_x, (first + i) * kK + 64, 0, bar);
-      };
-      const int head = min(n_stages, a.depth);
-      // Ahead of the wait for the kernel before: prepared weights (written by prepare only) are
-      // copied, 16-bit weights, which that kernel might have written, only drawn into L2.
+    if (lane < a.depth) {
+      ptx::mbar_init(&ctl.full[lane], 1);
+      ptx::mbar_init(&ctl.empty[lane], kWarps);
+    }
+    ptx::fence_barrier_init();
+    __syncwarp();
+  }
+  chain_release();
+  // The ranks meet here before they write to one another, and it costs nothing to arrive early.
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+
+  bool ok = true;
+  const int share = kOut / ranks, width = kTileM / ranks;   // outputs and weight rows of one rank
+  if (warp == kWarps) {
+    const bool leader = ptx::elect_one();
+    auto load_w = [&](int i) {
+      const int slot = i % a.depth, k = first + i;
+      uint8_t* dst = smem + slot * kStage;
+      uint64_t* bar = &ctl.full[slot];
+      ptx::mbar_arrive_expect_tx(bar, kStage);
+      if (kW4) {
+        ptx::bulk_g2s(dst, a.wq + ((size_t)m_tile * a.stages + k) * kWBytes, kWBytes, bar);
+      } else if (kGated) {
+        ptx::tma_load_2d(dst, &map_w, k * kK, m_tile * 64, bar);
+        ptx::tma_load_2d(dst + kWBytes / 2, &map_w, k * kK, a.up_row + m_tile * 64, bar);
+      } else {
+        ptx::tma_load_2d(dst, &map_w, k * kK, m_tile * kTileM, bar);
+      }
+    };
+    auto load_x = [&](int i) {
+      const int slot = i % a.depth, k = first + i;
+      uint8_t* dst = smem + slot * kStage + kWBytes;
+      ptx::tma_load_2d(dst, &map_x, k * kK, 0, &ctl.full[slot]);
+      if (kW4) ptx::tma_load_2d(dst + kNT * 1024, &map_x, k * kK + 64, 0, &ctl.full[slot]);
+    };
+    // Ahead of the wait for the kernel before: prepared weights (written by prepare only) are
+    // copied, 16-bit weights, which that kernel might have written, only drawn into L2.
+    const int head = min(n_stages, a.depth);
+    if (leader) {
       for (int i = 0; i < head; ++i) {
         if (kW4) {
-          ptx::mbar_arrive_expect_tx(&ctl.full[i], kStage);
-          load_w(i, &ctl.full[i]);
-        } else if (kGated) {
-          prefetch_tile(&map_w, (first + i) * kK, m_tile * 64);
-          prefetch_tile(&map_w, (first + i) * kK, a.up_row + m_tile * 64);
+          load_w(i);
         } else {
-          prefetch_tile(&map_w, (first + i) * kK, m_tile * kTileM);
+          prefetch_tile(&map_w, (first + i) * kK, m_tile * kOut);
+          if (kGated) prefetch_tile(&map_w, (first + i) * kK, a.up_row + m_tile * 64);
         }
       }
       chain_wait();
-      for (int i = 0; i < n_stages; ++i) {
-        const int slot = i % a.depth;
-        if (i >= a.depth && !ptx::mbar_wait(&ctl.empty[slot], ((i / a.depth) & 1) ^ 1)) {
+      for (int i = 0; i < head; ++i) {
+        if (!kW4) load_w(i);
+        load_x(i);
+      }
+    }
+    __syncwarp();
+    __syncthreads();      // the barriers are initialised: the consumers may wait on them
+    if (leader)
+      for (int i = head; i < n_stages; ++i) {
+        if (!ptx::mbar_wait(&ctl.empty[i % a.depth], ((i / a.depth) & 1) ^ 1)) {
           ok = false;
           break;
         }
-        if (!kW4 || i >= a.depth) {
-          ptx::mbar_arrive_expect_tx(&ctl.full[slot], kStage);
-          load_w(i, &ctl.full[slot]);
-        }
-        load_x(i, &ctl.full[slot]);
+        load_w(i);
+        load_x(i);
       }
-    }
+    __syncwarp();
   } else {
+    constexpr int kSets = kNT == 1 ? 2 : 1;   // neighbouring MMAs should not wait for each other
+    float acc[kSets][kNT][4];
+#pragma unroll
+    for (int h = 0; h < kSets; ++h)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[h][n][i] = 0.f;
+    __syncthreads();
+
     const int g = lane >> 2, t = lane & 3, r0 = warp * 16 + g;
     int slot = 0;
     uint32_t phase = 0;
     for (int i = 0; i < n_stages; ++i) {
-      if (!warp_wait(&ctl.full[slot], phase)) {
-        ok = false;
-        break;
-      }
+      // after an expired wait the warp runs on, together, over what is there
+      if (ok && !ptx::mbar_wait(&ctl.full[slot], phase)) ok = false;
+      __syncwarp();
       const uint8_t* w = smem + slot * kStage;
       const uint8_t* xb = w + kWBytes;
       if (kW4) {
+        // lane t's codes are k = 32 t .. 32 t + 31, word j eight of them
         const uint4 c0 = lds16(w + r0 * kRowCodeBytes + 16 * code_slot(r0, t));
         const uint4 c1 = lds16(w + (r0 + 8) * kRowCodeBytes + 16 * code_slot(r0 + 8, t));
+        const uint8_t* sc = w + kTileCodeBytes + r0 * kRowScaleBytes + 2 * t;
         uint32_t s0[2], s1[2];
-        expand_scales<kHalf>(*reinterpret_cast<const uint16_t*>(w + kTileCodeBytes + r0 * kRowScaleBytes + 2 * t), s0[0], s0[1]);
-        expand_scales<kHalf>(*reinterpret_cast<const uint16_t*>(w + kTileCodeBytes + (r0 + 8) * kRowScaleBytes + 2 * t), s1[0],
-                             s1[1]);
+        expand_scales<kHalf>(*reinterpret_cast<const uint16_t*>(sc), s0[0], s0[1]);
+        expand_scales<kHalf>(*reinterpret_cast<const uint16_t*>(sc + 8 * kRowScaleBytes), s1[0], s1[1]);
         const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {   // lane t's codes are k = 32 t .. 32 t + 31, word j eight of them
+        for (int j = 0; j < 4; ++j) {
           uint4 b[kNT];
 #pragma unroll
           for (int n = 0; n < kNT; ++n) b[n] = box_piece(xb + (t >> 1) * kNT * 1024, 8 * n + g, (t & 1) * 4 + j);
@@ -169,19 +186,20 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
           dequant_word<kHalf>(w1[j], s1[j >> 1], a.m16, a.m64, hi);
 #pragma unroll
           for (int n = 0; n < kNT; ++n) {
-            mma16816<kHalf>(acc[n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
-            mma16816<kHalf>(acc[n], lo[2], hi[2], lo[3], hi[3], b[n].z, b[n].w);
+            mma16816<kHalf>(acc[0][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
+            mma16816<kHalf>(acc[kSets - 1][n], lo[2], hi[2], lo[3], hi[3], b[n].z, b[n].w);
           }
         }
       } else {
+        // lane t's pieces are k = 16 t .. 16 t + 15
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {   // lane t's pieces are k = 16 t .. 16 t + 15
+        for (int j = 0; j < 2; ++j) {
           const uint4 lo = box_piece(w, r0, 2 * t + j), hi = box_piece(w, r0 + 8, 2 * t + j);
 #pragma unroll
           for (int n = 0; n < kNT; ++n) {
             const uint4 b = box_piece(xb, 8 * n + g, 2 * t + j);
-            mma16816<kHalf>(acc[n], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
-            mma16816<kHalf>(acc[n], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+            mma16816<kHalf>(acc[0][n], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+            mma16816<kHalf>(acc[kSets - 1][n], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
           }
         }
       }
@@ -193,66 +211,72 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
       }
     }
 #pragma unroll
-    for (int n = 0; n < kNT; ++n)
+    for (int h = 0; h < 2; ++h) {
+      const int row = r0 + 8 * h;
+      // output of the row, and whether it is the up half of a gated one
+      const int o = !kGated ? row : kW4 ? (row >> 5) * 16 + (row & 15) : row & 63;
+      const int up = !kGated ? 0 : kW4 ? (row >> 4) & 1 : row >> 6;
+      const int owner = o / share, at = owner * width + up * share + o - owner * share;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = 8 * n + 2 * t + (i & 1);
-        if (tok < a.tokens) sums[tok * kPitch + r0 + (i >> 1) * 8] = acc[n][i];
-      }
-    chain_wait();   // add is read and the outputs are written below
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int tok = 8 * n + 2 * t + i;
+          if (tok < toks) sums[tok * kPitch + at] = acc[0][n][2 * h + i] + (kSets > 1 ? acc[kSets - 1][n][2 * h + i] : 0.f);
+        }
+    }
   }
   if (!ok) give_up(a.error_flag);
   __syncwarp();
-  if (ranks > 1)
-    cluster_sync();
-  else
-    __syncthreads();
-
-  // Outputs of the tile: kOut per token, this rank's share of them.
-  constexpr int kOut = kGated ? kTileM / 2 : kTileM;
-  const int share = kOut / ranks;
+  chain_wait();   // add is read and the outputs are written below
+  __syncthreads();
   const float scale = kW4 ? __ldg(a.gs) * kUnscale<kHalf> : 1.f;
-  uint32_t base[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < ranks) base[k] = map_rank(sums, k);
-  auto total = [&](int tok, int row) {
-    float s = 0.f, v[8];
-    const uint32_t off = (tok * kPitch + row) * 4;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < ranks) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[k]) : "r"(base[k] + off) : "memory");
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < ranks) s += v[k];
-    return s * scale;
-  };
-  if (warp < kWarps) {
-    for (int i = threadIdx.x; i < share * a.tokens; i += 32 * kWarps) {
-      const int tok = i / share, o = rank * share + (i - tok * share);
-      const int col = m_tile * kOut + o;
-      if (col >= a.n_out) continue;
-      float v;
-      if (kGated) {
-        const int gate = kW4 ? (o >> 4) * 32 + (o & 15) : o;
-        const float ga = total(tok, gate), up = total(tok, gate + (kW4 ? 16 : 64));
-        if (!kW4 && a.ab) {
-          a.ab[(size_t)tok * 2 * a.n_out + col] = ga;
-          a.ab[(size_t)tok * 2 * a.n_out + a.n_out + col] = up;
-        }
-        v = silu_f(ga) * up;
-      } else {
-        v = total(tok, o);
-      }
-      if (a.add) v += load16(dtype, a.add + (size_t)tok * a.ld_add + col);
-      a.out[(size_t)tok * a.ldo + col] = round16(dtype, v);
+  if (ranks > 1) {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    const uint32_t mine = ptx::smem_u32(recv) + rank * toks * width * 4;
+    for (int i = threadIdx.x; i < toks * (kTileM / 4); i += kThreads) {
+      const int tok = i / (kTileM / 4), at = i % (kTileM / 4) * 4, owner = at / width;
+      const float4 v = *reinterpret_cast<const float4*>(sums + tok * kPitch + at);
+      uint32_t to;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(mine), "r"(owner));
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + (tok * width + at - owner * width) * 4),
+                   "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                   : "memory");
     }
-  }
-  if (ranks > 1) {   // the other ranks read this one's sums
-    __syncwarp();
     cluster_sync();
+  }
+
+  const float* from = ranks > 1 ? recv : sums;
+  const int tok_pitch = ranks > 1 ? width : kPitch;
+  for (int i = threadIdx.x; i < share * toks; i += kThreads) {
+    const int tok = i / share, o = i - tok * share;
+    const int col = m_tile * kOut + rank * share + o;
+    if (col >= a.n_out) continue;
+    float add = 0.f;
+    if (a.add) add = load16(dtype, a.add + (size_t)tok * a.ld_add + col);
+    const float* p = from + tok * tok_pitch + o;
+    float v = 0.f, up = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < ranks) {
+        v += p[k * toks * width];
+        if (kGated) up += p[k * toks * width + share];
+      }
+    v *= scale;
+    if (kGated) {
+      up *= scale;
+      if (!kW4 && a.ab) {
+        a.ab[(size_t)tok * 2 * a.n_out + col] = v;
+        a.ab[(size_t)tok * 2 * a.n_out + a.n_out + col] = up;
+      }
+      v = silu_f(v) * up;
+    }
+    a.out[(size_t)tok * a.ldo + col] = round16(dtype, v + add);
   }
 }
+
+// Shared memory beside the ring: the sums twice, the barriers and alignment.
+size_t rest_bytes(int tokens) { return 1024 + (size_t)4 * (kTileM + kPitch) * tokens + sizeof(Ctl); }
 
 // CTAs to aim for: about two on every SM keep enough copies in flight.
 constexpr int kTargetCtas = 2 * 148;
@@ -264,11 +288,10 @@ int launch(FewArgs a, int m_tiles, const CUtensorMap& mx, const CUtensorMap& mw,
   a.ranks = 1;
   while (a.ranks < 8 && m_tiles * a.ranks * 2 <= kTargetCtas && a.stages >= 4 * a.ranks) a.ranks *= 2;
   a.stages_per_rank = (a.stages + a.ranks - 1) / a.ranks;
-  const size_t rest = 1024 + sizeof(Ctl) + (size_t)4 * kPitch * a.tokens;
-  a.depth = (int)((kCtaBytes - rest) / kStage);
+  a.depth = (int)((kCtaBytes - rest_bytes(a.tokens)) / kStage);
   if (a.depth > kMaxDepth) a.depth = kMaxDepth;
   if (a.depth > a.stages_per_rank) a.depth = a.stages_per_rank;
-  const size_t smem = rest + (size_t)a.depth * kStage;
+  const size_t smem = rest_bytes(a.tokens) + (size_t)a.depth * kStage;
   static bool set[64] = {};  // per device: the attribute belongs to its context
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -306,7 +329,6 @@ int box_tokens(int tokens) { return tokens <= 8 ? 8 : tokens <= 16 ? 16 : 32; }
 int launch_few_w4(const LinearArgs& l, int dtype, bool gated, int* error_flag, cudaStream_t st) {
   FewArgs a{};
   a.wq = l.wq;
-  a.wsf = l.wsf;
   a.gs = l.gs;
   a.add = l.add;
   a.ld_add = l.ld_add;
@@ -337,11 +359,11 @@ int launch_few_dense(const DenseGemm& g, cudaStream_t st) {
   a.up_row = a.n_out;
   a.stages = (g.k + 63) / 64;
   a.error_flag = g.error_flag;
+  const int rows = gated ? 64 : kTileM;
   CUtensorMap mx, mw;
   int rc = make_operand_map(&mx, g.a, g.m, g.k, g.dtype, box_tokens(g.m));
-  if (!rc) rc = make_operand_map(&mw, g.b, g.n, g.k, g.dtype, gated ? 64 : kTileM);
+  if (!rc) rc = make_operand_map(&mw, g.b, g.n, g.k, g.dtype, rows);
   if (rc) return rc;
-  const int rows = gated ? 64 : kTileM;
   return launch_sized<false>(a, g.dtype, gated, (a.n_out + rows - 1) / rows, mx, mw, st);
 }
 

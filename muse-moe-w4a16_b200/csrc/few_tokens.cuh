@@ -5,12 +5,11 @@
 
 namespace muse {
 
-// The most tokens of a few-token call.
+// The most tokens of these calls.
 constexpr int kFewTokens = 32;
 
 struct FewArgs {
-  const uint8_t* wq;      // NVFP4: prepared codes, scales and the global scale
-  const uint8_t* wsf;
+  const uint8_t* wq;      // NVFP4: prepared tiles and the global scale
   const float* gs;
   const uint16_t* add;
   long long ld_add;
@@ -19,7 +18,7 @@ struct FewArgs {
   float* ab;              // gated 16-bit weights: pre-activations to keep, or null
   int tokens, n_out, up_row;
   int stages;             // stages of K: 128 codes or 64 16-bit columns
-  int ranks, stages_per_rank, depth;  // set by the launch
+  int ranks, stages_per_rank, depth;  // cluster size, stages of one rank, ring depth
   uint32_t m16, m64;
   int* error_flag;
 };

@@ -92,9 +92,10 @@ extern "C" int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int
   g.mode = kGate;
   g.out = ws + l.h, g.ldo = inter;
   g.ab = ab;
-  // up to kFewTokens tokens the weights are streamed, beyond the tensor-core pairs take over
+  // few tokens: the weights are streamed; beyond, the tensor-core pairs take over
   const auto product = tokens <= kFewTokens ? launch_few_dense : launch_dense_gemm;
-  if ((rc = product(g, (cudaStream_t)stream))) return rc;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if ((rc = product(g, st))) return rc;
   g.a = {ws + l.h, inter, true};
   g.b = {w2, ld2, true};
   g.n = hidden, g.k = inter;
@@ -102,7 +103,7 @@ extern "C" int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int
   g.out = out, g.ldo = hidden;
   g.ab = nullptr;
   g.add = add, g.ld_add = ld_add;
-  return product(g, (cudaStream_t)stream);
+  return product(g, st);
 }
 
 extern "C" int muse_moe_ffn_backward(const void* dy, long long ldy, const void* x, long long ldx, int dtype, int tokens,

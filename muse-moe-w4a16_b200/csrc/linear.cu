@@ -4,9 +4,10 @@
 //   y[t, n] = gs * sum_k x[t, k] * e2m1[n, k] * e4m3[n, k / 16]     (+ add[t, n])
 //   gated:  y[t, i] = silu(a) * b,  a, b = the products with gate row i and up row i
 //
-// The weight is kept in the tile order of layout.cuh (rows padded to 128, K to 128 with zero
-// codes), the routed experts' own format, so that sixteen rows of a 128-code chunk are 1 KiB in
-// a row and a code pair drops into a bf16x2 with one logic op.
+// The weight is kept in the routed experts' tile order (layout.cuh: 128 rows x 128 codes, permuted
+// so that a code pair drops into a bf16x2 with one logic op), rows and K padded with zero codes, and
+// each tile's scales behind its codes: a tile is one copy, and the tiles of one row range follow
+// one another along K.
 #undef MUSE_TRACE  // these kernels record no stamps
 #include "few_tokens.cuh"
 #include "kernels.cuh"
@@ -21,7 +22,7 @@ namespace {
 // in a w13 tile; `gate_up` is I, padded to 64 rows per half on its own.
 __global__ void __launch_bounds__(kTileM)
 prepare_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int cols,
-                      int gate_up, uint8_t* __restrict__ codes_out, uint8_t* __restrict__ scales_out) {
+                      int gate_up, uint8_t* __restrict__ out) {
   const int kc = blockIdx.x, m = blockIdx.y, r = threadIdx.x;
   const int k_chunks = gridDim.x;
   int src = m * kTileM + r;
@@ -32,8 +33,8 @@ prepare_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
     src = (r & 16) ? gate_up + j : j;
   }
   const size_t tile = (size_t)m * k_chunks + kc;
-  uint8_t* dst = codes_out + tile * kTileCodeBytes + (size_t)r * kRowCodeBytes;
-  uint8_t* sdst = scales_out + tile * kTileScaleBytes + (size_t)r * kRowScaleBytes;
+  uint8_t* dst = out + tile * kLinearTileBytes + r * kRowCodeBytes;
+  uint8_t* sdst = out + tile * kLinearTileBytes + kTileCodeBytes + r * kRowScaleBytes;
   const uint8_t* c = codes + (size_t)src * (cols / 2) + (size_t)kc * kRowCodeBytes;
   const uint8_t* s = scales + (size_t)src * (cols / 16) + (size_t)kc * kRowScaleBytes;
   const int blocks = row_ok ? min(8, cols / 16 - kc * 8) : 0;  // 16-code blocks inside the matrix
@@ -64,26 +65,22 @@ bool misaligned(const void* p, unsigned to) { return reinterpret_cast<uintptr_t>
 
 using namespace muse;
 
-extern "C" int muse_moe_linear_prepared_size(int rows, int cols, int gated, size_t* code_bytes, size_t* scale_bytes) {
-  if (!code_bytes || !scale_bytes) return MUSE_ERR_INVALID_ARGUMENT;
+extern "C" int muse_moe_linear_prepared_size(int rows, int cols, int gated, size_t* bytes) {
+  if (!bytes) return MUSE_ERR_INVALID_ARGUMENT;
   const int rc = check_linear(rows, cols, gated);
   if (rc) return rc;
-  const size_t n = (size_t)padded_rows_of(rows, gated) * padded(cols, kChunkK);
-  *code_bytes = n / 2;
-  *scale_bytes = n / kBlock;
+  *bytes = (size_t)(padded_rows_of(rows, gated) / kTileM) * (padded(cols, kChunkK) / kChunkK) * kLinearTileBytes;
   return MUSE_OK;
 }
 
 extern "C" int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int cols, int gated,
-                                       uint8_t* w_out, uint8_t* w_sf_out, muse_stream_t stream) {
+                                       uint8_t* out, muse_stream_t stream) {
   const int rc = check_linear(rows, cols, gated);
   if (rc) return rc;
-  if (!w || !w_sf || !w_out || !w_sf_out || misaligned(w, 8) || misaligned(w_out, 16) || misaligned(w_sf_out, 16))
-    return MUSE_ERR_INVALID_ARGUMENT;
+  if (!w || !w_sf || !out || misaligned(w, 8) || misaligned(out, 16)) return MUSE_ERR_INVALID_ARGUMENT;
   const dim3 grid(padded(cols, kChunkK) / kChunkK, padded_rows_of(rows, gated) / kTileM);
   if (grid.y > 65535) return MUSE_ERR_UNSUPPORTED_SHAPE;
-  prepare_linear_kernel<<<grid, kTileM, 0, (cudaStream_t)stream>>>(w, w_sf, rows, cols, gated ? rows / 2 : 0, w_out,
-                                                                   w_sf_out);
+  prepare_linear_kernel<<<grid, kTileM, 0, (cudaStream_t)stream>>>(w, w_sf, rows, cols, gated ? rows / 2 : 0, out);
   return last_launch_status();
 }
 
@@ -92,14 +89,14 @@ extern "C" int muse_moe_linear_workspace_size(int tokens, int rows, int cols, in
   const int rc = check_linear(rows, cols, gated);
   if (rc) return rc;
   if (tokens < 0) return MUSE_ERR_INVALID_ARGUMENT;
-  *bytes = tokens > kFewTokens
-               ? linear_gemm_scratch_bytes(tokens, padded_rows_of(rows, gated), padded(cols, kChunkK) / kChunkK)
-               : 0;
+  *bytes = tokens <= kFewTokens
+               ? 0
+               : linear_gemm_scratch_bytes(tokens, padded_rows_of(rows, gated), padded(cols, kChunkK) / kChunkK);
   return MUSE_OK;
 }
 
 extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int rows, int cols, int gated,
-                                  const uint8_t* wp, const uint8_t* w_sfp, const float* w_gs, const void* add,
+                                  const uint8_t* wp, const float* w_gs, const void* add,
                                   long long ld_add, void* out, long long ldo, void* workspace,
                                   size_t workspace_bytes, muse_stream_t stream) {
   int rc = check_linear(rows, cols, gated);
@@ -107,12 +104,11 @@ extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int t
   const int n_out = gated ? rows / 2 : rows;
   if (tokens < 0 || (dtype != kBf16 && dtype != kFp16)) return MUSE_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return MUSE_OK;
-  if (!x || !wp || !w_sfp || !w_gs || !out || misaligned(x, 16) || ldx % 8 || misaligned(wp, 16) ||
-      misaligned(w_sfp, 16) || (tokens > 1 && (ldx < cols || ldo < n_out || (add && ld_add < n_out))))
+  if (!x || !wp || !w_gs || !out || misaligned(x, 16) || ldx % 8 || misaligned(wp, 16) ||
+      (tokens > 1 && (ldx < cols || ldo < n_out || (add && ld_add < n_out))))
     return MUSE_ERR_INVALID_ARGUMENT;
   LinearArgs a{};
   a.wq = wp;
-  a.wsf = w_sfp;
   a.gs = w_gs;
   a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;

@@ -1,8 +1,8 @@
 // y = x . W^T with a prepared NVFP4 weight for more than a few tokens, on tcgen05 CTA pairs.
 //
 // Swap-AB: 256 weight rows per pair are the MMA's M, up to 256 tokens its N, so a decode batch
-// wastes no rows of M. Per 128-code chunk a CTA copies its 128 rows' codes and scales (9 KiB, one
-// bulk copy each) into a six-deep ring; sixteen warps turn them into exact 16-bit weights in
+// wastes no rows of M. Per 128-code chunk a CTA copies its 128 rows' codes and scales (one bulk
+// copy of 9 KiB) into a six-deep ring; sixteen warps turn them into exact 16-bit weights in
 // registers and write them as the K-major swizzled A operand (thread = weight row, one 128-byte
 // row of 64 k each); B is x by TMA, each CTA half of the tokens. Weights are dequantised once per
 // 256 tokens, which at ~140 instructions per thread and 64 k fits under the 512 clocks the MMAs
@@ -24,7 +24,7 @@ constexpr int kMaxStages = 9;
 constexpr int kABytes = kTileM * 128;
 constexpr int kRingBytes = 5 * 2 * kABytes;  // 64-k stages: A (16 KiB) and half of B (64 bytes a token)
 constexpr int kCodes = 6;                    // code ring: 128-code chunks of 9 KiB
-constexpr int kCodeBytes = kTileCodeBytes + kTileScaleBytes;
+constexpr int kCodeBytes = kLinearTileBytes;
 constexpr int kMaxBn = 256;
 constexpr int kPatch = 32 * 64;              // an epilogue warp's outputs of 32 tokens, 64 bytes each
 constexpr int kDeqWarp0 = 4, kEpiWarp0 = 20, kThreads = 768;
@@ -201,8 +201,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
           uint8_t* dst = codes + q.slot * kCodeBytes;
           const size_t tile = (size_t)m * k_chunks + c;
           ptx::mbar_arrive_expect_tx(&ctl.code_full[q.slot], kCodeBytes);
-          ptx::bulk_g2s(dst, a.l.wq + tile * kTileCodeBytes, kTileCodeBytes, &ctl.code_full[q.slot]);
-          ptx::bulk_g2s(dst + kTileCodeBytes, a.l.wsf + tile * kTileScaleBytes, kTileScaleBytes, &ctl.code_full[q.slot]);
+          ptx::bulk_g2s(dst, a.l.wq + tile * kLinearTileBytes, kLinearTileBytes, &ctl.code_full[q.slot]);
           q.next(kCodes);
         }
       }

@@ -8,9 +8,11 @@
 
 namespace muse {
 
+// A prepared tile: 128 rows' codes of 128 k, then their scales.
+constexpr int kLinearTileBytes = kTileCodeBytes + kTileScaleBytes;
+
 struct LinearArgs {
-  const uint8_t* wq;
-  const uint8_t* wsf;
+  const uint8_t* wq;         // prepared tiles
   const float* gs;
   const uint16_t* x;
   long long ldx;

@@ -80,14 +80,13 @@ def prepare_linear(weight: LinearWeights, gated: bool = False) -> dict:
     codes, scales = w.contiguous(), sf.contiguous().view(torch.uint8)
     if codes.data_ptr() % 8:
         codes = codes.clone()
-    nc, ns = ctypes.c_size_t(0), ctypes.c_size_t(0)
-    _lib.call("muse_moe_linear_prepared_size", N, K, int(gated), ctypes.byref(nc), ctypes.byref(ns))
-    out = torch.empty(nc.value, dtype=torch.uint8, device=dev)
-    out_sf = torch.empty(ns.value, dtype=torch.uint8, device=dev)
+    size = ctypes.c_size_t(0)
+    _lib.call("muse_moe_linear_prepared_size", N, K, int(gated), ctypes.byref(size))
+    out = torch.empty(size.value, dtype=torch.uint8, device=dev)
     with _on(dev):
         _lib.call("muse_moe_prepare_linear", codes.data_ptr(), scales.data_ptr(), N, K, int(gated),
-                  out.data_ptr(), out_sf.data_ptr(), _stream(dev))
-    return {"w": out, "w_sf": out_sf, "w_gs": gs.to(device=dev, dtype=torch.float32).reshape(1).clone(),
+                  out.data_ptr(), _stream(dev))
+    return {"w": out, "w_gs": gs.to(device=dev, dtype=torch.float32).reshape(1).clone(),
             "rows": N, "cols": K, "gated": bool(gated), "n_out": N // 2 if gated else N}
 
 
@@ -134,8 +133,8 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     with _on(dev):
         _lib.call("muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, int(state["gated"]),
-                  state["w"].data_ptr(), state["w_sf"].data_ptr(), state["w_gs"].data_ptr(), add_ptr, ld_add,
-                  out.data_ptr(), n_out, ws.data_ptr() if n else None, n, _stream(dev))
+                  state["w"].data_ptr(), state["w_gs"].data_ptr(), add_ptr, ld_add, out.data_ptr(),
+                  n_out, ws.data_ptr() if n else None, n, _stream(dev))
     return out
 
 

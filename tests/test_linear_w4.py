@@ -28,24 +28,24 @@ def test_cpu_tensors_are_refused(pkg):
 @pytest.mark.parametrize("rows,cols,gated,code", [(0, 64, 0, -1), (8, 0, 0, -1), (7, 64, 1, -1), (8, 64, 2, -1),
                                                   (8, 24, 0, -2), (1 << 25, 64, 0, -2)])
 def test_prepared_size_refuses(pkg, rows, cols, gated, code):
-    a, b = ctypes.c_size_t(), ctypes.c_size_t()
-    assert pkg.load_library().muse_moe_linear_prepared_size(rows, cols, gated, ctypes.byref(a), ctypes.byref(b)) == code
+    n = ctypes.c_size_t()
+    assert pkg.load_library().muse_moe_linear_prepared_size(rows, cols, gated, ctypes.byref(n)) == code
 
 
 @pytest.mark.parametrize("rows,cols,gated,n", [(1, 16, 0, 128 * 128), (128, 128, 0, 128 * 128), (129, 144, 0, 256 * 256),
                                                (2, 16, 1, 128 * 128), (130, 16, 1, 256 * 128)])
 def test_prepared_size(pkg, rows, cols, gated, n):
-    a, b = ctypes.c_size_t(), ctypes.c_size_t()
-    assert pkg.load_library().muse_moe_linear_prepared_size(rows, cols, gated, ctypes.byref(a), ctypes.byref(b)) == 0
-    assert (a.value, b.value) == (n // 2, n // 16)
+    size = ctypes.c_size_t()
+    assert pkg.load_library().muse_moe_linear_prepared_size(rows, cols, gated, ctypes.byref(size)) == 0
+    assert size.value == n // 2 + n // 16
 
 
 def test_entry_refuses_before_any_launch(pkg):
     lib = pkg.load_library()
     call = lambda **k: lib.muse_moe_linear_w4(*[{**dict(  # noqa: E731
-        x=256, ldx=64, dtype=0, tokens=2, rows=32, cols=64, gated=0, wp=256, sf=256, gs=256, add=None, ld_add=0,
+        x=256, ldx=64, dtype=0, tokens=2, rows=32, cols=64, gated=0, wp=256, gs=256, add=None, ld_add=0,
         out=256, ldo=32, ws=256, bytes=1 << 30, stream=None), **k}[n] for n in ("x", "ldx", "dtype", "tokens", "rows", "cols", "gated", "wp",
-                                                        "sf", "gs", "add", "ld_add", "out", "ldo", "ws", "bytes", "stream")])
+                                                        "gs", "add", "ld_add", "out", "ldo", "ws", "bytes", "stream")])
     assert call(tokens=0) == 0
     for bad in (dict(tokens=-1), dict(dtype=2), dict(x=None), dict(wp=None), dict(gs=None), dict(out=None),
                 dict(x=264), dict(ldx=68), dict(ldx=56), dict(ldo=31), dict(add=256, ld_add=31)):
