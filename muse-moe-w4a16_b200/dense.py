@@ -9,7 +9,6 @@ synchronisation; so calls can be captured in a CUDA graph after one eager call.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import TypedDict
@@ -17,7 +16,7 @@ from typing import TypedDict
 import torch
 
 from . import _lib
-from .layer import _require_cuda, _stream
+from .layer import _require_cuda
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -32,9 +31,23 @@ def _bad(message: str) -> _lib.MuseError:
     return _lib.MuseError(_lib.MUSE_ERR_INVALID_ARGUMENT, message)
 
 
-def _on(device: torch.device):
-    """Context with `device` current (the kernels launch on the current device)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+# Handle of a device's current stream, without the Stream object that torch.cuda.current_stream
+# builds (2 us of a call's host time, as much as its launch) where torch has the direct form.
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(index: int, name: str, *args) -> None:
+    """An entry point on device `index` and its current stream (kernels launch on the current device)."""
+    if torch.cuda.current_device() == index:
+        _lib.call(name, *args, _current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _current_stream(index))
+
+
+def _scratch(n: int, device: torch.device) -> torch.Tensor:
+    return torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device)
 
 
 def _same(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) -> None:
@@ -49,6 +62,8 @@ def _rows(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
     allow it, else a contiguous copy."""
     if t.dim() != 2:
         t = t.reshape(-1, width)
+    if t.is_contiguous() and not t.data_ptr() % 16:
+        return t, width
     ld = t.stride(0) if t.shape[0] > 1 else width
     if t.stride(1) != 1 or ld % 8 or ld < width or t.data_ptr() % 16:
         t = t.contiguous()
@@ -83,9 +98,7 @@ def prepare_linear(weight: LinearWeights, gated: bool = False) -> dict:
     size = ctypes.c_size_t(0)
     _lib.call("muse_moe_linear_prepared_size", N, K, int(gated), ctypes.byref(size))
     out = torch.empty(size.value, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _lib.call("muse_moe_prepare_linear", codes.data_ptr(), scales.data_ptr(), N, K, int(gated),
-                  out.data_ptr(), _stream(dev))
+    _call(dev.index, "muse_moe_prepare_linear", codes.data_ptr(), scales.data_ptr(), N, K, int(gated), out.data_ptr())
     return {"w": out, "w_gs": gs.to(device=dev, dtype=torch.float32).reshape(1).clone(),
             "rows": N, "cols": K, "gated": bool(gated), "n_out": N // 2 if gated else N}
 
@@ -103,38 +116,41 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
     one, plus `add` (same shape) if given. x is bf16 or fp16, and so are add and the result; any
     number of rows. Sums in fp32, one rounding. Inference only: it has no gradient."""
     _require_cuda(x, "x")
-    K, n_out, dev = state["cols"], state["n_out"], x.device
+    K, n_out, w, dev = state["cols"], state["n_out"], state["w"], x.device
     dtype = _DTYPES.get(x.dtype)
     if dtype is None:
         raise _bad(f"x must be bfloat16 or float16, got {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] != K:
-        raise _bad(f"x {tuple(x.shape)} does not end in the weight's {K} columns")
-    if state["w"].device != dev:
-        raise _bad(f"the weight is on {state['w'].device}, x on {dev}")
+    shape = x.shape
+    if not shape or shape[-1] != K:
+        raise _bad(f"x {tuple(shape)} does not end in the weight's {K} columns")
+    if w.device != dev:
+        raise _bad(f"the weight is on {w.device}, x on {dev}")
     if torch.is_grad_enabled() and (x.requires_grad or (add is not None and add.requires_grad)):
         raise _bad("linear_w4 has no gradient: call it under torch.no_grad()")
-    shape = x.shape[:-1] + (n_out,)
     x2, ldx = _rows(x, K)
     T = x2.shape[0]
+    if len(shape) == 2:
+        shape = (T, n_out)
+    else:
+        shape = shape[:-1] + (n_out,)
     add_ptr, ld_add = None, 0
     if add is not None:
         _same(add, "add", dev, x.dtype)
         if add.shape != shape:
             raise _bad(f"add must be {tuple(shape)}, got {tuple(add.shape)}")
         add2 = add if add.dim() == 2 else add.reshape(-1, n_out)
-        if add2.stride(1) != 1 or (T > 1 and add2.stride(0) < n_out):
+        if not add2.is_contiguous() and (add2.stride(1) != 1 or (T > 1 and add2.stride(0) < n_out)):
             add2 = add2.contiguous()
         add_ptr, ld_add = add2.data_ptr(), add2.stride(0)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        out = x.new_empty(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         raise _bad(f"out must be a contiguous {x.dtype} {tuple(shape)} on {dev}")
-    n = _linear_workspace(T, state["rows"], K, int(state["gated"]))
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    with _on(dev):
-        _lib.call("muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, int(state["gated"]),
-                  state["w"].data_ptr(), state["w_gs"].data_ptr(), add_ptr, ld_add, out.data_ptr(),
-                  n_out, ws.data_ptr() if n else None, n, _stream(dev))
+    gated = 1 if state["gated"] else 0
+    n = _linear_workspace(T, state["rows"], K, gated)
+    ws = _scratch(n, dev) if n else None
+    _call(dev.index, "muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, gated, w.data_ptr(),
+          state["w_gs"].data_ptr(), add_ptr, ld_add, out.data_ptr(), n_out, ws.data_ptr() if n else None, n)
     return out
 
 
@@ -151,7 +167,7 @@ def _ffn_forward(x, w13, w2, add, keep: bool):
     dev, dtype = x.device, x.dtype
     x2, ldx = _rows(x, H)
     T = x2.shape[0]
-    out = torch.empty(x.shape, dtype=dtype, device=dev)
+    out = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     ab = torch.empty((T, 2 * I), dtype=torch.float32, device=dev) if keep else None
     if T == 0:
         return out, ab
@@ -159,11 +175,10 @@ def _ffn_forward(x, w13, w2, add, keep: bool):
     w2, ld2 = _rows(w2, I)
     add2, ld_add = (None, 0) if add is None else _rows(add, H)
     n = _ffn_workspace(T, H, I, 0)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _lib.call("muse_moe_ffn_forward", x2.data_ptr(), ldx, _DTYPES[dtype], T, H, I, w13.data_ptr(), ld13,
-                  w2.data_ptr(), ld2, None if add is None else add2.data_ptr(), ld_add, out.data_ptr(),
-                  ab.data_ptr() if keep else None, ws.data_ptr(), n, _stream(dev))
+    ws = _scratch(n, dev)
+    _call(dev.index, "muse_moe_ffn_forward", x2.data_ptr(), ldx, _DTYPES[dtype], T, H, I, w13.data_ptr(), ld13,
+          w2.data_ptr(), ld2, None if add is None else add2.data_ptr(), ld_add, out.data_ptr(),
+          ab.data_ptr() if keep else None, ws.data_ptr(), n)
     return out, ab
 
 
@@ -195,12 +210,11 @@ class _GatedFfn(torch.autograd.Function):
                 w13, ld13 = _rows(w13, H)
                 w2, ld2 = _rows(w2, I)
                 n = _ffn_workspace(T, H, I, 1)
-                ws = torch.empty(n, dtype=torch.uint8, device=dev)
-                with _on(dev):
-                    _lib.call("muse_moe_ffn_backward", dy2.data_ptr(), ldy, x2.data_ptr(), ldx, _DTYPES[x.dtype], T,
-                              H, I, w13.data_ptr(), ld13, w2.data_ptr(), ld2, ab.data_ptr(),
-                              dx.data_ptr() if need_x else None, dw13.data_ptr() if need_13 else None,
-                              dw2.data_ptr() if need_2 else None, ws.data_ptr(), n, _stream(dev))
+                ws = _scratch(n, dev)
+                _call(dev.index, "muse_moe_ffn_backward", dy2.data_ptr(), ldy, x2.data_ptr(), ldx, _DTYPES[x.dtype], T,
+                      H, I, w13.data_ptr(), ld13, w2.data_ptr(), ld2, ab.data_ptr(),
+                      dx.data_ptr() if need_x else None, dw13.data_ptr() if need_13 else None,
+                      dw2.data_ptr() if need_2 else None, ws.data_ptr(), n)
         return dx, dw13, dw2, dy if need_add else None
 
 
