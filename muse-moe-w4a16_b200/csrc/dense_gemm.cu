@@ -13,9 +13,9 @@
 // they lie (64-wide boxes, "MN-major" descriptors): no transposed copy is made.
 // Six ring stages of 64 k; two accumulators of 256 columns, so a tile's epilogue (eight warps)
 // overlaps the next tile's MMAs. Pairs are persistent and walk a static tile list, eight row tiles
-// to a group, so that the tiles in flight share their operands in L2. With too few tiles for the
-// pairs K is split and fp32 partials are summed, in split order, by a second kernel: results do
-// not depend on timing.
+// to a group, so that the tiles in flight share their operands in L2. Tiles that do not
+// fill a wave of the pairs are split along K and their fp32 partials summed, in split order, by a
+// second kernel: results do not depend on timing.
 // In the gate product the leader's half of B is gate rows and its peer's half the matching up
 // rows, so one thread holds a and b of the same element.
 // Bound by: the tensor pipe for many tokens, weight bytes for few.
@@ -52,8 +52,9 @@ static_assert(kSmem <= 232448, "shared memory of one CTA");
 
 struct Args {
   int m, n, inter;                    // inter: I of the gate modes (0 otherwise)
-  int bn, tiles_m, tiles_n, splits, kb_total, kb_per_split;
-  int dtype, partial;                 // partial: write fp32 sums to `partials` instead
+  int bn, tiles_m, tiles_n, kb_total;
+  int whole, splits, kb_per_split;    // tiles done whole; the others (the tail) in `splits` items each
+  int dtype;
   uint32_t idesc;
   uint32_t tx_bytes;                  // both CTAs' bytes per stage
   void* out;
@@ -67,21 +68,33 @@ struct Args {
 };
 
 struct Tile {
-  int m0, n0, kb0, kb1, split;
+  int m0, n0, kb0, kb1;
+  float* partial;  // an item of the tail: its 256 x bn block of partial sums (else null)
 };
-// Work item -> tile: splits innermost, then kGroupM row tiles per column tile.
-__device__ __forceinline__ Tile tile_of(const Args& a, int w) {
-  Tile t;
-  const int idx = w / a.splits;
-  t.split = w - idx * a.splits;
+// Tile `idx` of the raster: kGroupM row tiles per column tile. n0 is the column tile's index.
+__device__ __forceinline__ void raster(const Args& a, int idx, int& m0, int& n0) {
   const int group = idx / (kGroupM * a.tiles_n);
   const int first = group * kGroupM;
   const int rows = min(kGroupM, a.tiles_m - first);
   const int r = idx - group * kGroupM * a.tiles_n;
-  t.m0 = (first + r % rows) * 2 * kBm;
-  t.n0 = r / rows;                         // column tile index
-  t.kb0 = t.split * a.kb_per_split;
-  t.kb1 = min(a.kb_total, t.kb0 + a.kb_per_split);
+  m0 = (first + r % rows) * 2 * kBm;
+  n0 = r / rows;
+}
+// Work items: the whole tiles, then the tail's, splits innermost.
+__device__ __forceinline__ Tile tile_of(const Args& a, int w) {
+  Tile t;
+  int idx = w;
+  t.kb0 = 0;
+  t.kb1 = a.kb_total;
+  t.partial = nullptr;
+  if (w >= a.whole && a.splits > 1) {
+    const int item = w - a.whole, split = item % a.splits;
+    idx = a.whole + item / a.splits;
+    t.kb0 = split * a.kb_per_split;
+    t.kb1 = min(a.kb_total, t.kb0 + a.kb_per_split);
+    t.partial = a.partials + (size_t)item * 2 * kBm * a.bn;
+  }
+  raster(a, idx, t.m0, t.n0);
   return t;
 }
 
@@ -91,8 +104,10 @@ __device__ __forceinline__ void store4(int dtype, void* base, long long ld, int 
   p.y = pack16(dtype, v.z, v.w);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + (size_t)row * ld + col) = p;
 }
-__device__ __forceinline__ float4 add4(int dtype, const void* base, long long ld, int row, int col, float4 v) {
-  const uint2 p = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + (size_t)row * ld + col));
+__device__ __forceinline__ uint2 load4(const void* base, long long ld, int row, int col) {
+  return __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + (size_t)row * ld + col));
+}
+__device__ __forceinline__ float4 add4(int dtype, uint2 p, float4 v) {
   const float2 lo = unpack16(dtype, p.x), hi = unpack16(dtype, p.y);
   return make_float4(v.x + lo.x, v.y + lo.y, v.z + hi.x, v.w + hi.y);
 }
@@ -115,6 +130,28 @@ __device__ __forceinline__ void dgate4(const Args& p, int row, int col, float4 d
   store4(p.dtype, p.out, p.ldo, row, p.inter + col, db);
   store4(p.dtype, p.h_out, p.inter, row, col, h);
 }
+
+// What a patch is combined with, one 4-column piece for each of a lane's eight rows: the addend, or a
+// and b.
+template <int kMode> struct SideInput {
+  uint2 add[8];
+  __device__ __forceinline__ void load(const Args& p, int i, int row, int col, bool more) {
+    if (p.add && more && row < p.m && col < p.n) add[i] = load4(p.add, p.ld_add, row, col);
+  }
+};
+template <> struct SideInput<kDGate> {
+  float4 a[8], b[8];
+  __device__ __forceinline__ void load(const Args& p, int i, int row, int col, bool more) {
+    if (more && row < p.m && col < p.n) {
+      const float* at = p.ab + (size_t)row * 2 * p.inter + col;
+      a[i] = __ldg(reinterpret_cast<const float4*>(at));
+      b[i] = __ldg(reinterpret_cast<const float4*>(at + p.inter));
+    }
+  }
+};
+template <> struct SideInput<kGate> {
+  __device__ __forceinline__ void load(const Args&, int, int, int, bool) {}
+};
 
 // 32 x 32 fp32 patch of one warp: thread = row writes its 32 columns, then lane l reads columns
 // 4 (l % 8) .. + 3 of row 4 i + l / 8. 16-byte pieces are swizzled by the row: no bank conflicts.
@@ -139,7 +176,7 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int total = a.tiles_m * a.tiles_n * a.splits;
+  const int total = a.whole + (a.tiles_m * a.tiles_n - a.whole) * a.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -257,6 +294,13 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
     for (int w = pair; w < total; w += pairs, ++it) {
       const Tile t = tile_of(a, w);
       const int buf = it & 1;
+      // what the first patch is combined with, fetched while its sums are still being taken
+      SideInput<kMode> side;
+      if (!t.partial) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          side.load(a, i, t.m0 + rank * kBm + quarter * 32 + 4 * i + rr, t.n0 * a.bn + 32 * half + cc, true);
+      }
       if (!warp_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
         ok = false;
         break;
@@ -284,38 +328,31 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
           tmem_ld32(acc + pairs_cols + c, u);
           ptx::tmem_wait_ld();
           const bool in = col < a.inter;
-          if (a.partial || a.ab) {
-            float* to = a.partial ? a.partials + (size_t)t.split * a.m * a.n : a.ab;
+          if (t.partial) {
+            float* to = t.partial + (size_t)(rank * kBm + quarter * 32) * a.bn + c + cc;
+            each(g, [&](int r, float4 v) { *reinterpret_cast<float4*>(to + (size_t)(r - row0) * a.bn) = v; });
+            each(u, [&](int r, float4 v) { *reinterpret_cast<float4*>(to + (size_t)(r - row0) * a.bn + pairs_cols) = v; });
+            continue;
+          }
+          if (a.ab) {
             each(g, [&](int r, float4 v) {
-              if (in) *reinterpret_cast<float4*>(to + (size_t)r * a.n + col) = v;
+              if (in) *reinterpret_cast<float4*>(a.ab + (size_t)r * a.n + col) = v;
             });
             each(u, [&](int r, float4 v) {
-              if (in) *reinterpret_cast<float4*>(to + (size_t)r * a.n + a.inter + col) = v;
+              if (in) *reinterpret_cast<float4*>(a.ab + (size_t)r * a.n + a.inter + col) = v;
             });
           }
-          if (!a.partial) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) g[j] = silu_f(g[j]) * u[j];
-            each(g, [&](int r, float4 v) {
-              if (in) store4(a.dtype, a.out, a.ldo, r, col, v);
-            });
-          }
+          for (int j = 0; j < 32; ++j) g[j] = silu_f(g[j]) * u[j];
+          each(g, [&](int r, float4 v) {
+            if (in) store4(a.dtype, a.out, a.ldo, r, col, v);
+          });
         }
       } else if (rows) {
         for (int c = 32 * half; c < a.bn; c += 64) {
           const int col = t.n0 * a.bn + c + cc;
           if (t.n0 * a.bn + c >= a.n) break;
           const bool in = col < a.n;
-          float4 ga[8], gb[8];
-          if (kMode == kDGate && !a.partial) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (in && row0 + 4 * i + rr < a.m) {
-                const float* at = a.ab + (size_t)(row0 + 4 * i + rr) * 2 * a.inter + col;
-                ga[i] = __ldg(reinterpret_cast<const float4*>(at));
-                gb[i] = __ldg(reinterpret_cast<const float4*>(at + a.inter));
-              }
-          }
           float v[32];
           tmem_ld32(acc + c, v);
           ptx::tmem_wait_ld();
@@ -325,16 +362,21 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = row0 + 4 * i + rr;
-            if (!in || r >= a.m) continue;
             float4 x = patch_get(patch, lane, i);
-            if (a.partial) {
-              *reinterpret_cast<float4*>(a.partials + ((size_t)t.split * a.m + r) * a.n + col) = x;
-            } else if (kMode == kDGate) {
-              dgate4(a, r, col, x, ga[i], gb[i]);
-            } else {
-              if (a.add) x = add4(a.dtype, a.add, a.ld_add, r, col, x);
-              store4(a.dtype, a.out, a.ldo, r, col, x);
+            if (t.partial) {
+              if (r < a.m && in)
+                *reinterpret_cast<float4*>(t.partial + (size_t)(r - t.m0) * a.bn + c + cc) = x;
+              continue;
             }
+            if (r < a.m && in) {
+              if constexpr (kMode == kDGate) {
+                dgate4(a, r, col, x, side.a[i], side.b[i]);
+              } else if constexpr (kMode == kStore) {
+                if (a.add) x = add4(a.dtype, side.add[i], x);
+                store4(a.dtype, a.out, a.ldo, r, col, x);
+              }
+            }
+            side.load(a, i, r, col + 64, c + 64 < a.bn);   // the next patch's
           }
         }
       }
@@ -353,20 +395,27 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Sum of the splits' partials, in split order, with the mode's epilogue. One float4 of columns
-// per thread; the partials were just written and are read from L2.
+// Sums of the tail's partials, in split order, with the mode's epilogue: a block takes eight rows of
+// a tile, a thread four columns at a time. The partials were just written and are read from L2.
+constexpr int kReduceRows = 8;
+
 template <int kMode>
 __global__ void __launch_bounds__(256) dense_reduce(const Args a) {
   chain_release();
   chain_wait();
-  const int width = kMode == kGate ? a.inter : a.n;
+  int m0, n0;
+  raster(a, a.whole + blockIdx.x, m0, n0);
+  const int width = kMode == kGate ? a.bn >> 1 : a.bn;
   const int q = width >> 2;
-  const size_t plane = (size_t)a.m * a.n;
-  const size_t items = (size_t)a.m * q;
-  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < items; i += (size_t)gridDim.x * blockDim.x) {
-    const int row = (int)(i / q), col = (int)(i - (size_t)row * q) * 4;
-    auto sum = [&](int c) {
-      const float* p = a.partials + (size_t)row * a.n + c;
+  const size_t plane = (size_t)2 * kBm * a.bn;
+  const float* tile = a.partials + (size_t)blockIdx.x * a.splits * plane;
+  const int last = kMode == kGate ? a.inter : a.n;
+  for (int i = threadIdx.x; i < kReduceRows * q; i += 256) {
+    const int r = blockIdx.y * kReduceRows + i / q, c = i % q * 4;
+    const int row = m0 + r, col = n0 * width + c;
+    if (row >= a.m || col >= last) continue;
+    auto sum = [&](int at) {
+      const float* p = tile + (size_t)r * a.bn + at;
       float4 s = __ldcg(reinterpret_cast<const float4*>(p));
 #pragma unroll 4
       for (int k = 1; k < a.splits; ++k) {
@@ -375,9 +424,9 @@ __global__ void __launch_bounds__(256) dense_reduce(const Args a) {
       }
       return s;
     };
-    float4 x = sum(col);
+    float4 x = sum(c);
     if (kMode == kGate) {
-      const float4 u = sum(a.inter + col);
+      const float4 u = sum(width + c);
       if (a.ab) {
         float* at = a.ab + (size_t)row * a.n + col;
         *reinterpret_cast<float4*>(at) = x;
@@ -390,7 +439,7 @@ __global__ void __launch_bounds__(256) dense_reduce(const Args a) {
       dgate4(a, row, col, x, __ldg(reinterpret_cast<const float4*>(at)),
              __ldg(reinterpret_cast<const float4*>(at + a.inter)));
     } else {
-      if (a.add) x = add4(a.dtype, a.add, a.ld_add, row, col, x);
+      if (a.add) x = add4(a.dtype, load4(a.add, a.ld_add, row, col), x);
       store4(a.dtype, a.out, a.ldo, row, col, x);
     }
   }
@@ -399,13 +448,16 @@ __global__ void __launch_bounds__(256) dense_reduce(const Args a) {
 constexpr int kPairs = 74;  // 148 SMs, two to a pair
 
 struct Plan {
-  int bn, tiles_m, tiles_n, splits, kb_total, kb_per_split;
+  int bn, tiles_m, tiles_n, kb_total, whole, splits, kb_per_split;
+  int tail() const { return splits > 1 ? tiles_m * tiles_n - whole : 0; }
 };
 
-// Tile width and split of K, from the sizes alone: the least estimated time in SM clocks. A stage
+// Tile width, and the split of K for the tail: the tiles that do not fill a wave of all pairs are cut
+// along K into one item per pair (448 tiles, as a 4096-token step has, would else pay a seventh wave
+// for its last four). Chosen from the sizes alone, by the least estimated time in SM clocks. A stage
 // of a pair costs the larger of its MMA time (2 bn clocks for 64 k) and its loads ((128 + bn / 2)
-// rows of 128 B at ~60 B per clock and SM from L2); a tile's start and last epilogue ~2500; a split adds the
-// reduction's launch and its partials' way through L2 (~2 KB per clock over the chip).
+// rows of 128 B at ~60 B per clock and SM from L2); a tile's start and last epilogue ~2500; a split
+// adds the reduction's launch and its partials' way through L2 (~2 KB per clock over the chip).
 Plan make_plan(int m, int n, int k, int mode, bool b_k_major) {
   Plan best{};
   double best_cost = 0;
@@ -419,14 +471,15 @@ Plan make_plan(int m, int n, int k, int mode, bool b_k_major) {
     p.tiles_n = (n + bn - 1) / bn;
     if (mode == kGate) p.tiles_n = (n / 2 + bn / 2 - 1) / (bn / 2);
     p.kb_total = kb;
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n, tail = tiles % kPairs;
     const double stage = 2.0 * bn > (128 + bn / 2) * 128 / 60.0 ? 2.0 * bn : (128 + bn / 2) * 128 / 60.0;
-    for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= kPairs && kb / s >= 4)); ++s) {
+    for (int s = 1; s <= 16 && (s == 1 || (tail * s <= kPairs && kb / s >= 4 && tail > 0)); ++s) {
       p.kb_per_split = (kb + s - 1) / s;
       p.splits = (kb + p.kb_per_split - 1) / p.kb_per_split;
-      const double waves = (double)((tiles * p.splits + kPairs - 1) / kPairs);
-      double cost = waves * p.kb_per_split * stage + 2500;
-      if (p.splits > 1) cost += 4000 + 8.0 * m * n * p.splits / 2000;
+      p.whole = (int)(p.splits > 1 ? tiles - tail : tiles);
+      double cost = (double)(tiles / kPairs) * kb * stage + 2500;
+      if (tail) cost += p.kb_per_split * stage;
+      if (p.splits > 1) cost += 4000 + 8.0 * 256 * bn * tail * p.splits / 2000;
       if (best.bn == 0 || cost < best_cost) {
         best = p;
         best_cost = cost;
@@ -448,14 +501,12 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, cudaStre
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) set[dev] = true;
   }
-  const long long total = (long long)a.tiles_m * a.tiles_n * a.splits;
-  const int pairs = total < kPairs ? (int)total : kPairs;
+  const int tail = a.splits > 1 ? a.tiles_m * a.tiles_n - a.whole : 0;
+  const int total = a.whole + tail * a.splits;
+  const int pairs = total < kPairs ? total : kPairs;
   int rc = launch_chained(dense_gemm<kAMn, kBMn, kMode>, dim3(2 * pairs), dim3(kThreads), kSmem, st, 2, ma, mb, a);
-  if (rc || !a.partial) return rc;
-  const size_t items = (size_t)a.m * ((kMode == kGate ? a.inter : a.n) >> 2);
-  const size_t blocks = (items + 255) / 256;
-  return launch_chained(dense_reduce<kMode>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st,
-                        1, a);
+  if (rc || !tail) return rc;
+  return launch_chained(dense_reduce<kMode>, dim3(tail, 2 * kBm / kReduceRows), dim3(256), 0, st, 1, a);
 }
 
 }  // namespace
@@ -491,12 +542,12 @@ int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k,
 size_t dense_scratch_bytes(int m, int n, int k, int mode, bool b_k_major) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
   const Plan p = make_plan(m, n, k, mode, b_k_major);
-  return p.splits > 1 ? (size_t)4 * p.splits * m * n : 0;
+  return (size_t)4 * p.tail() * p.splits * 2 * kBm * p.bn;
 }
 
 int launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
   const Plan p = make_plan(g.m, g.n, g.k, g.mode, g.b.k_major);
-  if ((long long)p.tiles_m * p.tiles_n * p.splits > 0x7FFFFFFFLL) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  if ((long long)p.tiles_m * p.tiles_n > (1 << 30)) return MUSE_ERR_UNSUPPORTED_SHAPE;
   Args a{};
   a.m = g.m;
   a.n = g.n;
@@ -504,11 +555,11 @@ int launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
   a.bn = p.bn;
   a.tiles_m = p.tiles_m;
   a.tiles_n = p.tiles_n;
-  a.splits = p.splits;
   a.kb_total = p.kb_total;
+  a.whole = p.whole;
+  a.splits = p.splits;
   a.kb_per_split = p.kb_per_split;
   a.dtype = g.dtype;
-  a.partial = p.splits > 1;
   const uint32_t type = g.dtype == kBf16 ? 1u : 0u;  // operand format: 0 f16, 1 bf16
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((g.a.k_major ? 0u : 1u) << 15) |
             ((g.b.k_major ? 0u : 1u) << 16) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(2 * kBm >> 4) << 24);
@@ -521,7 +572,7 @@ int launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
   a.h_out = g.h_out;
   a.partials = g.partials;
   a.error_flag = g.error_flag;
-  if (a.partial && !g.partials) return MUSE_ERR_WORKSPACE_TOO_SMALL;
+  if (p.tail() && !g.partials) return MUSE_ERR_WORKSPACE_TOO_SMALL;
   CUtensorMap ma, mb;
   int rc = make_operand_map(&ma, g.a, g.m, g.k, g.dtype, kBm);
   if (!rc) rc = make_operand_map(&mb, g.b, g.n, g.k, g.dtype, p.bn / 2);
