@@ -376,7 +376,11 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
                 store4(a.dtype, a.out, a.ldo, r, col, x);
               }
             }
-            side.load(a, i, r, col + 64, c + 64 < a.bn);   // the next patch's
+          }
+          // the next patch's, all after the last use: loads and uses in turn would wait for one another
+          if (!t.partial) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) side.load(a, i, row0 + 4 * i + rr, col + 64, c + 64 < a.bn);
           }
         }
       }
