@@ -55,6 +55,17 @@ int launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
 // 64 m x 64 k, 128-byte swizzle, zeros out of bounds.
 int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k, int dtype, int box);
 
+// Map of gated weights [gate rows; up rows] (K-major) as [inter / 8][2][8] rows: a box is 64 k x eight
+// gate and the eight matching up rows x eight such groups, 128 rows in that order.
+int make_gated_map(CUtensorMap* map, const DenseOperand& o, int inter, int k, int dtype);
+
+// The forward products (modes kStore and kGate without ab, both operands along k) with the weights on
+// the MMA's M side (swap_gemm.cu), and both forms' estimated times in SM clocks.
+double dense_cost(int m, int n, int k, int mode, bool b_k_major);
+double swap_dense_cost(int m, int n, int k);
+size_t swap_dense_scratch_bytes(int m, int n, int k);
+int launch_swap_dense(const DenseGemm& g, cudaStream_t stream);
+
 // ---- 16-bit conversions shared by the dense kernels
 
 // Logistic function and silu with the fast division (2 steps of 2^-24; its range ends at 2^126, where

@@ -462,7 +462,7 @@ struct Plan {
 // of a pair costs the larger of its MMA time (2 bn clocks for 64 k) and its loads ((128 + bn / 2)
 // rows of 128 B at ~60 B per clock and SM from L2); a tile's start and last epilogue ~2500; a split
 // adds the reduction's launch and its partials' way through L2 (~2 KB per clock over the chip).
-Plan make_plan(int m, int n, int k, int mode, bool b_k_major) {
+Plan make_plan(int m, int n, int k, int mode, bool b_k_major, double* cost_out = nullptr) {
   Plan best{};
   double best_cost = 0;
   const int kb = (k + kBk - 1) / kBk;
@@ -490,6 +490,7 @@ Plan make_plan(int m, int n, int k, int mode, bool b_k_major) {
       }
     }
   }
+  if (cost_out) *cost_out = best_cost;
   return best;
 }
 
@@ -541,6 +542,27 @@ int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k,
              const_cast<void*>(o.ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? MUSE_OK : MUSE_ERR_INVALID_ARGUMENT;
+}
+
+int make_gated_map(CUtensorMap* map, const DenseOperand& o, int inter, int k, int dtype) {
+  const auto encode = encode_fn();
+  if (!encode) return MUSE_ERR_NO_DEVICE;
+  const cuuint64_t row = (cuuint64_t)o.ld * 2;
+  cuuint64_t dims[4] = {(cuuint64_t)k, 8, 2, (cuuint64_t)inter / 8};
+  cuuint64_t strides[3] = {row, row * inter, row * 8};
+  cuuint32_t boxes[4] = {64, 8, 2, 8};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      encode(map, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+             const_cast<void*>(o.ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MUSE_OK : MUSE_ERR_INVALID_ARGUMENT;
+}
+
+double dense_cost(int m, int n, int k, int mode, bool b_k_major) {
+  double cost;
+  make_plan(m, n, k, mode, b_k_major, &cost);
+  return cost;
 }
 
 size_t dense_scratch_bytes(int m, int n, int k, int mode, bool b_k_major) {

@@ -57,12 +57,6 @@ __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_c
 __device__ __forceinline__ uint4 box_piece(const uint8_t* box, int r, int p) {
   return lds16(box + r * 128 + ((p ^ (r & 7)) << 4));
 }
-__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int c0, int c1) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
-               "r"(c0), "r"(c1)
-               : "memory");
-}
-
 template <bool kW4, int kNT, bool kHalf, bool kGated>
 __global__ void __launch_bounds__(kThreads)
 few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const FewArgs a) {

@@ -1,17 +1,22 @@
-// y = x . W^T with a prepared NVFP4 weight for more than a few tokens, on tcgen05 CTA pairs.
+// y = x . W^T with the weight rows on the MMA's M side ("swap-AB"), on tcgen05 CTA pairs: the product
+// of a prepared NVFP4 weight with more than a few tokens, and the feed-forward block's forward
+// products of 16-bit weights where that beats tokens on the M side (dense_gemm.cu).
 //
-// Swap-AB: 256 weight rows per pair are the MMA's M, up to 256 tokens its N, so a decode batch
-// wastes no rows of M. Per 128-code chunk a CTA copies its 128 rows' codes and scales (one bulk
-// copy of 9 KiB) into a six-deep ring; sixteen warps turn them into exact 16-bit weights in
-// registers and write them as the K-major swizzled A operand (thread = weight row, one 128-byte
-// row of 64 k each); B is x by TMA, each CTA half of the tokens. Weights are dequantised once per
-// 256 tokens, which at ~140 instructions per thread and 64 k fits under the 512 clocks the MMAs
-// of a 256-token stage take. Accumulators are double buffered in tensor memory; the epilogue
-// reads them as matrix fragments and turns them over (rows are weight rows, y's rows are tokens)
-// with transposed matrix stores into shared memory, so that global stores run along y's rows. A
-// gated tile holds 16 gate rows and the 16 matching up rows per warp: one thread has both.
+// 256 weight rows per pair are M and up to 256 tokens N, in steps of 32, so a batch of any size
+// wastes little. B is x by TMA, each CTA half of the tokens. A is
+//   16-bit weights: by TMA. Gated: a view of w13 as [I / 8][gate, up][8] rows puts eight gate rows
+//   and the eight matching up rows next to one another, in one box.
+//   NVFP4: per 128-code chunk a CTA copies its 128 rows' codes and scales (one bulk copy of 9 KiB)
+//   into a six-deep ring; sixteen warps turn them into exact 16-bit weights in registers and write
+//   them as the K-major swizzled A operand (thread = weight row, one 128-byte row of 64 k each).
+//   Weights are dequantised once per 256 tokens, which fits under the 512 clocks of a stage's MMAs.
+// Accumulators are double buffered in tensor memory; the epilogue reads them as matrix fragments
+// and turns them over (rows are weight rows, y's rows are tokens) with transposed matrix stores
+// into shared memory, so that global stores run along y's rows. Gated tiles hold gate and up rows
+// of an output in one thread's fragments.
 // With fewer tiles than pairs K is split; a second kernel adds the fp32 partials in split order.
-// Bound by weight bytes and the dequantisation for tens of tokens, by the tensor pipe for hundreds.
+// Bound by weight bytes (NVFP4: and the dequantisation) for tens of tokens, by the tensor pipe for
+// hundreds.
 #undef MUSE_TRACE  // these kernels record no stamps
 #include "kernels.cuh"
 #include "pair.cuh"
@@ -20,14 +25,17 @@
 namespace muse {
 namespace {
 
-constexpr int kMaxStages = 9;
+constexpr int kMaxStages = 12;
 constexpr int kABytes = kTileM * 128;
-constexpr int kRingBytes = 5 * 2 * kABytes;  // 64-k stages: A (16 KiB) and half of B (64 bytes a token)
 constexpr int kCodes = 6;                    // code ring: 128-code chunks of 9 KiB
 constexpr int kCodeBytes = kLinearTileBytes;
+// 64-k stages: A (16 KiB) and half of B (64 bytes a token).
+template <bool kW4> constexpr int kRingBytes = 5 * 2 * kABytes + (kW4 ? 0 : 3 * kABytes);
 constexpr int kMaxBn = 256;
 constexpr int kPatch = 32 * 64;              // an epilogue warp's outputs of 32 tokens, 64 bytes each
-constexpr int kDeqWarp0 = 4, kEpiWarp0 = 20, kThreads = 768;
+constexpr int kDeqWarp0 = 4;                 // warps 0-2: codes, MMA, TMA; then dequantisers; then the epilogue
+template <bool kW4> constexpr int kEpiWarp0 = kW4 ? 20 : 4;
+template <bool kW4> constexpr int kThreads = 32 * (kEpiWarp0<kW4> + 4);
 
 struct Ctl {
   uint64_t full[kMaxStages], empty[kMaxStages];
@@ -35,11 +43,12 @@ struct Ctl {
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem;
 };
-constexpr size_t kSmem = 1024 + (size_t)kRingBytes + (size_t)kCodes * kCodeBytes + 4 * kPatch + sizeof(Ctl);
-static_assert(kSmem <= 232448, "shared memory of one CTA");
+template <bool kW4>
+constexpr size_t kSmem = 1024 + (size_t)kRingBytes<kW4> + (kW4 ? kCodes * kCodeBytes : 0) + 4 * kPatch + sizeof(Ctl);
+static_assert(kSmem<true> <= 232448 && kSmem<false> <= 232448, "shared memory of one CTA");
 
 struct GemmPlan {
-  int bn, stages, tiles_m, tiles_n, splits, chunks_per_split;
+  int bn, stages, tiles_m, tiles_n, splits, units, units_per_split;  // units of K: 128 codes or 64 columns
 };
 
 struct Args {
@@ -56,7 +65,7 @@ struct Tile {
   int m_tile, tok0, c0, c1, split;
 };
 // Work item -> tile: splits innermost, then eight row tiles per token tile.
-__device__ __forceinline__ Tile tile_of(const GemmPlan& p, int k_chunks, int w, uint32_t rank) {
+__device__ __forceinline__ Tile tile_of(const GemmPlan& p, int w, uint32_t rank) {
   constexpr int kGroup = 8;
   Tile t;
   const int idx = w / p.splits;
@@ -67,8 +76,8 @@ __device__ __forceinline__ Tile tile_of(const GemmPlan& p, int k_chunks, int w, 
   const int r = idx - group * kGroup * p.tiles_n;
   t.m_tile = 2 * (first + r % rows) + (int)rank;
   t.tok0 = r / rows * p.bn;
-  t.c0 = t.split * p.chunks_per_split;
-  t.c1 = min(k_chunks, t.c0 + p.chunks_per_split);
+  t.c0 = t.split * p.units_per_split;
+  t.c1 = min(p.units, t.c0 + p.units_per_split);
   return t;
 }
 
@@ -83,6 +92,30 @@ struct Pos {
     }
   }
 };
+
+// 128 weight rows x 64 k of tile m_tile (16-bit weights) into shared memory, or into L2. Gated: eight
+// groups of eight gate and eight up rows.
+template <bool kGated>
+__device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* map, int k, int m_tile, uint32_t bar) {
+  if (kGated)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(k), "r"(0), "r"(m_tile * 8), "r"(bar)
+        : "memory");
+  else
+    tma_pair(dst, map, k, m_tile * kTileM, bar);
+}
+template <bool kGated>
+__device__ __forceinline__ void prefetch_weights(const CUtensorMap* map, int k, int m_tile) {
+  if (kGated)
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %2, %3}];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(k), "r"(0), "r"(m_tile * 8)
+                 : "memory");
+  else
+    prefetch_tile(map, k, m_tile * kTileM);
+}
 
 // 16-byte piece `p` of token row `tok` of a patch; pieces are swizzled so that eight token rows of
 // one piece, and the four pieces of two rows, lie in different banks.
@@ -140,27 +173,27 @@ struct PatchIo {
   }
 };
 
-template <bool kHalf, bool kGated>
-__global__ void __launch_bounds__(kThreads, 1)
-linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
+template <bool kW4, bool kHalf, bool kGated>
+__global__ void __launch_bounds__(kThreads<kW4>, 1)
+swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Args a) {
+  constexpr int kUnit = kW4 ? 2 : 1;   // stages of a unit
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* codes = smem + kRingBytes;
+  uint8_t* codes = smem + kRingBytes<kW4>;
   const int n_stages = a.p.stages, stage_bytes = kABytes + a.p.bn * 64;
-  uint8_t* patches = codes + kCodes * kCodeBytes;
+  uint8_t* patches = codes + (kW4 ? kCodes * kCodeBytes : 0);
   Ctl& ctl = *reinterpret_cast<Ctl*>(patches + 4 * kPatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int total = a.p.tiles_m * a.p.tiles_n * a.p.splits;
-  const int k_chunks = a.l.k_chunks;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stages; ++s) {
-      ptx::mbar_init(&ctl.full[s], 1 + 2 * 4);  // B bytes announced by the leader; A by four warps of each CTA
+      ptx::mbar_init(&ctl.full[s], kW4 ? 1 + 2 * 4 : 1);  // bytes announced by the leader; NVFP4's A by four warps of each CTA
       ptx::mbar_init(&ctl.empty[s], 1);
     }
-    for (int s = 0; s < kCodes; ++s) {
+    for (int s = 0; kW4 && s < kCodes; ++s) {
       ptx::mbar_init(&ctl.code_full[s], 1);
       ptx::mbar_init(&ctl.code_empty[s], 8);
     }
@@ -187,10 +220,10 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
   bool ok = true;
   if (warp == 0) {
     // Codes: written by prepare only, so they are fetched without waiting for the kernel before.
-    if (ptx::elect_one()) {
+    if (kW4 && ptx::elect_one()) {
       Pos q;
       for (int w = pair; w < total && ok; w += pairs) {
-        const Tile t = tile_of(a.p, k_chunks, w, rank);
+        const Tile t = tile_of(a.p, w, rank);
         // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
         const int m = min(t.m_tile, a.l.padded_rows / kTileM - 1);
         for (int c = t.c0; c < t.c1; ++c) {
@@ -199,7 +232,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
             break;
           }
           uint8_t* dst = codes + q.slot * kCodeBytes;
-          const size_t tile = (size_t)m * k_chunks + c;
+          const size_t tile = (size_t)m * a.p.units + c;
           ptx::mbar_arrive_expect_tx(&ctl.code_full[q.slot], kCodeBytes);
           ptx::bulk_g2s(dst, a.l.wq + tile * kLinearTileBytes, kLinearTileBytes, &ctl.code_full[q.slot]);
           q.next(kCodes);
@@ -211,7 +244,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
       Pos s;
       int it = 0;
       for (int w = pair; w < total && ok; w += pairs, ++it) {
-        const Tile t = tile_of(a.p, k_chunks, w, rank);
+        const Tile t = tile_of(a.p, w, rank);
         const int buf = it & 1;
         if (!ptx::mbar_wait(&ctl.acc_empty[buf], ((it >> 1) & 1) ^ 1)) {
           ok = false;
@@ -219,7 +252,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
         }
         ptx::tc_fence_after();
         const uint32_t d = tmem + buf * kMaxBn;
-        for (int n = 2 * t.c0; n < 2 * t.c1; ++n) {
+        for (int n = kUnit * t.c0; n < kUnit * t.c1; ++n) {
           if (!ptx::mbar_wait(&ctl.full[s.slot], s.phase)) {
             ok = false;
             break;
@@ -229,7 +262,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
           const uint64_t da = operand_desc<false>(sa), db = operand_desc<false>(sa + kABytes);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, n > 2 * t.c0 || j > 0);
+            mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, n > kUnit * t.c0 || j > 0);
           commit_pair(&ctl.empty[s.slot]);
           s.next(n_stages);
         }
@@ -238,19 +271,25 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
     }
   } else if (warp == 2) {
     if (ptx::elect_one()) {
+      if (!kW4 && pair < total) {
+        // 16-bit weights might have been written by the kernel before: only drawn into L2 ahead of it
+        const Tile t = tile_of(a.p, pair, rank);
+        for (int n = t.c0; n < min(t.c1, t.c0 + n_stages); ++n) prefetch_weights<kGated>(&map_w, n * 64, t.m_tile);
+      }
       chain_wait();
       Pos s;
       for (int w = pair; w < total && ok; w += pairs) {
-        const Tile t = tile_of(a.p, k_chunks, w, rank);
+        const Tile t = tile_of(a.p, w, rank);
         const int row = t.tok0 + (int)rank * (a.p.bn >> 1);
-        for (int n = 2 * t.c0; n < 2 * t.c1; ++n) {
+        for (int n = kUnit * t.c0; n < kUnit * t.c1; ++n) {
           if (!ptx::mbar_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
             ok = false;
             break;
           }
-          if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], 2 * a.b_bytes);
-          tma_pair(ptx::smem_u32(smem + s.slot * stage_bytes) + kABytes, &map_x, n * 64, row,
-                   map_rank(&ctl.full[s.slot], 0));
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], 2 * (a.b_bytes + (kW4 ? 0 : kABytes)));
+          const uint32_t dst = ptx::smem_u32(smem + s.slot * stage_bytes), bar = map_rank(&ctl.full[s.slot], 0);
+          if (!kW4) load_weights<kGated>(dst, &map_w, n * 64, t.m_tile, bar);
+          tma_pair(dst + kABytes, &map_x, n * 64, row, bar);
           s.next(n_stages);
         }
       }
@@ -260,7 +299,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
         s.next(n_stages);
       }
     }
-  } else if (warp >= kDeqWarp0 && warp < kEpiWarp0) {
+  } else if (kW4 && warp >= kDeqWarp0 && warp < kEpiWarp0<kW4>) {
     // four groups of four warps: group (p, h) takes half h of every second chunk
     const int h = ((warp - kDeqWarp0) >> 2) & 1;      // 64-k half of the chunk
     const int r = (warp & 3) * 32 + lane;             // weight row of the tile
@@ -268,7 +307,7 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
     Pos q, s;
     if (h) s.next(n_stages);
     for (int w = pair; w < total && ok; w += pairs) {
-      const Tile t = tile_of(a.p, k_chunks, w, rank);
+      const Tile t = tile_of(a.p, w, rank);
       for (int c = t.c0; c < t.c1; ++c, mine = !mine, q.next(kCodes), s.next(n_stages), s.next(n_stages)) {
         if (!mine) continue;
         if (!warp_wait(&ctl.code_full[q.slot], q.phase)) {
@@ -301,16 +340,16 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
         if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], 0));
       }
     }
-  } else if (warp >= kEpiWarp0) {
+  } else if (warp >= kEpiWarp0<kW4>) {
     chain_wait();
     const int quarter = warp & 3;
     const uint32_t lane_base = tmem + ((uint32_t)quarter << 21);
     constexpr int dtype = kHalf ? kFp16 : kBf16;
-    const float gs = __ldg(a.l.gs) * kUnscale<kHalf>;
-    uint8_t* patch = patches + (warp - kEpiWarp0) * kPatch;
+    const float gs = kW4 ? __ldg(a.l.gs) * kUnscale<kHalf> : 1.f;
+    uint8_t* patch = patches + (warp - kEpiWarp0<kW4>) * kPatch;
     int it = 0;
     for (int w = pair; w < total; w += pairs, ++it) {
-      const Tile t = tile_of(a.p, k_chunks, w, rank);
+      const Tile t = tile_of(a.p, w, rank);
       const int buf = it & 1;
       constexpr int kOut = kGated ? 16 : 32;              // outputs of the warp
       using Io = PatchIo<kOut>;
@@ -346,6 +385,21 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
         tmem_ld_frag(acc + c + (16u << 16), hi);
         ptx::tmem_wait_ld();
         const int tok0 = t.tok0 + c, toks = min(32, n_tok - c);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = 4 * b + i;
+            if (!kGated) {
+              lo[j] *= gs;
+              hi[j] *= gs;
+            } else if (kW4) {          // rows 0-15 gate, 16-31 up
+              lo[j] = silu_f(lo[j] * gs) * (hi[j] * gs);
+            } else if (i < 2) {        // rows 0-7 gate, 8-15 up; 16-23 gate, 24-31 up
+              lo[j] = silu_f(lo[j]) * lo[j + 2];
+              lo[j + 2] = silu_f(hi[j]) * hi[j + 2];
+            }
+          }
         __syncwarp();                                       // the patch's last readers are done
         if (adds) {
           Io::put(patch, lane, ahead);
@@ -360,25 +414,16 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float2 u = unpack16(dtype, f[i]);
-              if (kGated) {
-                lo[4 * b + 2 * i] = silu_f(lo[4 * b + 2 * i] * gs) * (hi[4 * b + 2 * i] * gs) + u.x;
-                lo[4 * b + 2 * i + 1] = silu_f(lo[4 * b + 2 * i + 1] * gs) * (hi[4 * b + 2 * i + 1] * gs) + u.y;
-              } else {
+              lo[4 * b + 2 * i] += u.x;
+              lo[4 * b + 2 * i + 1] += u.y;
+              if (!kGated) {
                 const float2 w2 = unpack16(dtype, f[2 + i]);
-                lo[4 * b + 2 * i] = lo[4 * b + 2 * i] * gs + u.x;
-                lo[4 * b + 2 * i + 1] = lo[4 * b + 2 * i + 1] * gs + u.y;
-                hi[4 * b + 2 * i] = hi[4 * b + 2 * i] * gs + w2.x;
-                hi[4 * b + 2 * i + 1] = hi[4 * b + 2 * i + 1] * gs + w2.y;
+                hi[4 * b + 2 * i] += w2.x;
+                hi[4 * b + 2 * i + 1] += w2.y;
               }
             }
           }
           __syncwarp();
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            lo[j] = kGated ? silu_f(lo[j] * gs) * (hi[j] * gs) : lo[j] * gs;
-            hi[j] *= gs;
-          }
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -407,23 +452,24 @@ linear_gemm(const __grid_constant__ CUtensorMap map_x, const Args a) {
 }
 
 // Sum of the splits' partials in split order, scale, gate and addend; one output per thread.
-template <bool kHalf, bool kGated>
-__global__ void __launch_bounds__(256) linear_reduce(const Args a) {
+template <bool kW4, bool kHalf, bool kGated>
+__global__ void __launch_bounds__(256) swap_reduce(const Args a) {
   chain_release();
   chain_wait();
   constexpr int dtype = kHalf ? kFp16 : kBf16;
-  const float gs = __ldg(a.l.gs) * kUnscale<kHalf>;
+  constexpr int kGroup = kW4 ? 16 : 8;   // gate rows in a row, then their up rows
+  const float gs = kW4 ? __ldg(a.l.gs) * kUnscale<kHalf> : 1.f;
   const size_t plane = (size_t)a.l.tokens * a.l.padded_rows;
   const size_t items = (size_t)a.l.tokens * a.l.n_out;
   for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < items; i += (size_t)gridDim.x * blockDim.x) {
     const int tok = (int)(i / a.l.n_out), o = (int)(i - (size_t)tok * a.l.n_out);
-    const int row = kGated ? (o >> 4) * 32 + (o & 15) : o;
+    const int row = kGated ? o / kGroup * 2 * kGroup + o % kGroup : o;
     const float* p = a.partials + (size_t)tok * a.l.padded_rows + row;
     float s = 0.f, u = 0.f;
 #pragma unroll 4
     for (int k = 0; k < a.p.splits; ++k) {
       s += __ldcg(p + k * plane);
-      if (kGated) u += __ldcg(p + k * plane + 16);
+      if (kGated) u += __ldcg(p + k * plane + kGroup);
     }
     float y = s * gs;
     if (kGated) y = silu_f(y) * (u * gs);
@@ -435,10 +481,13 @@ __global__ void __launch_bounds__(256) linear_reduce(const Args a) {
 constexpr int kPairs = 74;  // 148 SMs, two to a pair
 
 // Token tile and split of K from the sizes alone: the least estimated time in SM clocks. A 64-k
-// stage costs its MMAs (2 bn) or the ring's latency over its depth (~2600 from a freed stage over
-// dequantisation, cluster arrival, MMA and commit to the next free one); a tile's start and epilogue 2000 + 8 per token; a split the second
+// stage costs its MMAs (2 bn) or, NVFP4, the ring's latency over its depth (~2600 from a freed stage
+// over dequantisation, cluster arrival, MMA and commit to the next free one), 16 bits, its loads
+// (~60 B per clock and SM from L2); a tile's start and epilogue 2000 + 8 per token; a split the second
 // kernel's launch and the partials' way through L2 (~2 KB per clock over the chip).
-GemmPlan make_plan(int tokens, int padded_rows, int k_chunks) {
+template <bool kW4>
+GemmPlan make_plan(int tokens, int padded_rows, int units, double* cost_out = nullptr) {
+  constexpr int kUnit = kW4 ? 2 : 1;
   GemmPlan best{};
   double best_cost = 0;
   for (int bn = 32; bn <= 256; bn += 32) {
@@ -446,16 +495,17 @@ GemmPlan make_plan(int tokens, int padded_rows, int k_chunks) {
     p.bn = bn;
     p.tiles_m = (padded_rows + 255) / 256;
     p.tiles_n = (tokens + bn - 1) / bn;
+    p.units = units;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    p.stages = kRingBytes / (kABytes + bn * 64);
+    p.stages = kRingBytes<kW4> / (kABytes + bn * 64);
     if (p.stages > kMaxStages) p.stages = kMaxStages;
-    double stage = 2600.0 / p.stages;
+    double stage = kW4 ? 2600.0 / p.stages : (128 + bn / 2) * 128 / 60.0;
     if (2.0 * bn > stage) stage = 2.0 * bn;
-    for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= kPairs && k_chunks / s >= 2)); ++s) {
-      p.chunks_per_split = (k_chunks + s - 1) / s;
-      p.splits = (k_chunks + p.chunks_per_split - 1) / p.chunks_per_split;
+    for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= kPairs && kUnit * units / s >= 4)); ++s) {
+      p.units_per_split = (units + s - 1) / s;
+      p.splits = (units + p.units_per_split - 1) / p.units_per_split;
       const double waves = (double)((tiles * p.splits + kPairs - 1) / kPairs);
-      double cost = waves * (2 * p.chunks_per_split * stage) + 2000 + 8.0 * bn;
+      double cost = waves * (kUnit * p.units_per_split * stage) + 2000 + 8.0 * bn;
       if (p.splits > 1) cost += 4000 + 8.0 * tokens * padded_rows * p.splits / 2000;
       if (best.bn == 0 || cost < best_cost) {
         best = p;
@@ -463,55 +513,97 @@ GemmPlan make_plan(int tokens, int padded_rows, int k_chunks) {
       }
     }
   }
+  if (cost_out) *cost_out = best_cost;
   return best;
 }
 
-template <bool kHalf, bool kGated>
-int launch(const CUtensorMap& map, const Args& a, cudaStream_t st) {
+template <bool kW4, bool kHalf, bool kGated>
+int launch(const CUtensorMap& mx, const CUtensorMap& mw, const Args& a, cudaStream_t st) {
   static bool set[64] = {};  // per device: the attribute belongs to its context
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev >= 64 || !set[dev]) {
-    e = cudaFuncSetAttribute(linear_gemm<kHalf, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    e = cudaFuncSetAttribute(swap_gemm<kW4, kHalf, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<kW4>);
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) set[dev] = true;
   }
   const long long total = (long long)a.p.tiles_m * a.p.tiles_n * a.p.splits;
   const int pairs = total < kPairs ? (int)total : kPairs;
-  int rc = launch_chained(linear_gemm<kHalf, kGated>, dim3(2 * pairs), dim3(kThreads), kSmem, st, 2, map, a);
+  int rc = launch_chained(swap_gemm<kW4, kHalf, kGated>, dim3(2 * pairs), dim3(kThreads<kW4>), kSmem<kW4>, st, 2, mx, mw, a);
   if (rc || !a.partials) return rc;
   const size_t blocks = ((size_t)a.l.tokens * a.l.n_out + 255) / 256;
-  return launch_chained(linear_reduce<kHalf, kGated>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256),
+  return launch_chained(swap_reduce<kW4, kHalf, kGated>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256),
                         0, st, 1, a);
 }
+
+template <bool kW4>
+int launch_any(const LinearArgs& l, const GemmPlan& p, const CUtensorMap& mw, int dtype, bool gated, float* partials,
+               int* error_flag, cudaStream_t st) {
+  Args a{};
+  a.l = l;
+  a.p = p;
+  if ((long long)p.tiles_m * p.tiles_n * p.splits > 0x7FFFFFFFLL) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  const uint32_t type = dtype == kBf16 ? 1u : 0u;  // operand format: 0 f16, 1 bf16
+  a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+  a.b_bytes = (uint32_t)p.bn / 2 * 128;
+  auto vec = [](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
+  a.out_vec = vec(l.out, l.ldo);
+  a.add_vec = vec(l.add, l.ld_add);
+  a.partials = p.splits > 1 ? partials : nullptr;
+  a.error_flag = error_flag;
+  CUtensorMap mx;
+  const int rc = make_operand_map(&mx, DenseOperand{l.x, l.ldx, true}, l.tokens, l.cols, dtype, p.bn / 2);
+  if (rc) return rc;
+  if (dtype == kFp16) return gated ? launch<kW4, true, true>(mx, mw, a, st) : launch<kW4, true, false>(mx, mw, a, st);
+  return gated ? launch<kW4, false, true>(mx, mw, a, st) : launch<kW4, false, false>(mx, mw, a, st);
+}
+
+int padded_rows_of(const DenseGemm& g) { return (g.n + kTileM - 1) / kTileM * kTileM; }
 
 }  // namespace
 
 size_t linear_gemm_scratch_bytes(int tokens, int padded_rows, int k_chunks) {
-  const GemmPlan p = make_plan(tokens, padded_rows, k_chunks);
+  const GemmPlan p = make_plan<true>(tokens, padded_rows, k_chunks);
   return p.splits > 1 ? (size_t)4 * p.splits * tokens * padded_rows : 0;
 }
 
 int launch_linear_gemm(const LinearArgs& l, int dtype, bool gated, float* partials, int* error_flag, cudaStream_t st) {
-  Args a{};
-  a.l = l;
-  a.p = make_plan(l.tokens, l.padded_rows, l.k_chunks);
-  if ((long long)a.p.tiles_m * a.p.tiles_n * a.p.splits > 0x7FFFFFFFLL) return MUSE_ERR_UNSUPPORTED_SHAPE;
-  const uint32_t type = dtype == kBf16 ? 1u : 0u;
-  a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(a.p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
-  a.b_bytes = (uint32_t)a.p.bn / 2 * 128;
-  auto vec = [](const void* p, long long ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
-  a.out_vec = vec(l.out, l.ldo);
-  a.add_vec = vec(l.add, l.ld_add);
-  a.partials = a.p.splits > 1 ? partials : nullptr;
-  a.error_flag = error_flag;
-  CUtensorMap map;
-  const DenseOperand x{l.x, l.ldx, true};
-  const int rc = make_operand_map(&map, x, l.tokens, l.cols, dtype, a.p.bn / 2);
+  return launch_any<true>(l, make_plan<true>(l.tokens, l.padded_rows, l.k_chunks), CUtensorMap{}, dtype, gated, partials,
+                          error_flag, st);
+}
+
+double swap_dense_cost(int m, int n, int k) {
+  double cost;
+  make_plan<false>(m, (n + kTileM - 1) / kTileM * kTileM, (k + 63) / 64, &cost);
+  return cost;
+}
+
+size_t swap_dense_scratch_bytes(int m, int n, int k) {
+  const int rows = (n + kTileM - 1) / kTileM * kTileM;
+  const GemmPlan p = make_plan<false>(m, rows, (k + 63) / 64);
+  return p.splits > 1 ? (size_t)4 * p.splits * m * rows : 0;
+}
+
+int launch_swap_dense(const DenseGemm& g, cudaStream_t st) {
+  const bool gated = g.mode == kGate;
+  LinearArgs l{};
+  l.x = static_cast<const uint16_t*>(g.a.ptr);
+  l.ldx = g.a.ld;
+  l.add = static_cast<const uint16_t*>(g.add);
+  l.ld_add = g.ld_add;
+  l.out = static_cast<uint16_t*>(g.out);
+  l.ldo = g.ldo;
+  l.tokens = g.m;
+  l.cols = g.k;
+  l.n_out = gated ? g.n / 2 : g.n;
+  l.padded_rows = padded_rows_of(g);
+  CUtensorMap mw;
+  const int rc = gated ? make_gated_map(&mw, g.b, l.n_out, g.k, g.dtype)
+                       : make_operand_map(&mw, g.b, g.n, g.k, g.dtype, kTileM);
   if (rc) return rc;
-  if (dtype == kFp16) return gated ? launch<true, true>(map, a, st) : launch<true, false>(map, a, st);
-  return gated ? launch<false, true>(map, a, st) : launch<false, false>(map, a, st);
+  return launch_any<false>(l, make_plan<false>(g.m, l.padded_rows, (g.k + 63) / 64), mw, g.dtype, gated, g.partials,
+                           g.error_flag, st);
 }
 
 }  // namespace muse

@@ -1,5 +1,5 @@
 // In-register dequantisation of prepared NVFP4 code words (layout.cuh) and the launch interface
-// of the many-token 4-bit product (linear_gemm.cu).
+// of the many-token 4-bit product (swap_gemm.cu).
 #pragma once
 
 #include "dense.cuh"
