@@ -59,8 +59,8 @@ int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k,
 // gate and the eight matching up rows x eight such groups, 128 rows in that order.
 int make_gated_map(CUtensorMap* map, const DenseOperand& o, int inter, int k, int dtype);
 
-// The forward products (modes kStore and kGate without ab, both operands along k) with the weights on
-// the MMA's M side (swap_gemm.cu), and both forms' estimated times in SM clocks.
+// The forward products (modes kStore and kGate, both operands along k) with the weights on the MMA's
+// M side (swap_gemm.cu), and both forms' estimated times in SM clocks.
 double dense_cost(int m, int n, int k, int mode, bool b_k_major);
 double swap_dense_cost(int m, int n, int k);
 size_t swap_dense_scratch_bytes(int m, int n, int k);

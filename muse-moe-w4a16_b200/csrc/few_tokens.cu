@@ -4,8 +4,8 @@
 // A CTA takes 128 weight rows (gated 16-bit weights: 64 gate rows and the 64 matching up rows) and a
 // cluster of CTAs splits K. One thread copies the weights into a ring of shared memory, 128 codes
 // or 64 16-bit columns to a stage (one bulk copy of a tile, or a TMA box), and the same columns of
-// x (TMA; rows past the last token read as zeros). Eight warps multiply 16 rows each by mma.sync
-// m16n8k16: tokens are the 8-wide side, so one token wastes no weight traffic, and at 32 tokens the
+// x (TMA; rows past the last token read as zeros). Eight warps multiply 16 rows each (from nine
+// tokens on 32 rows and half of the k) by mma.sync m16n8k16: tokens are the 8-wide side, so one token wastes no weight traffic, and at 32 tokens the
 // matrix pipe still keeps up with HBM. Lanes read both operands as 16-byte pieces along k -- the order of k inside a
 // stage is the lanes' -- so nothing is shuffled. A CTA pushes its sums to the ranks that own the
 // outputs (16-byte stores to distributed shared memory, one cluster barrier), which add them in
@@ -142,17 +142,23 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
       }
     __syncwarp();
   } else {
+    // A warp takes 16 rows. Two token groups: 32 rows and half of the stage's k, which halves
+    // the reads of x per row (13 x 2048 x 7168: 11.9 to 9.5 us; with four groups the registers cost more).
+    constexpr int kMT = kNT == 2 ? 2 : 1;
     constexpr int kSets = kNT == 1 ? 2 : 1;   // neighbouring MMAs should not wait for each other
-    float acc[kSets][kNT][4];
+    float acc[kSets][kMT][kNT][4];
 #pragma unroll
     for (int h = 0; h < kSets; ++h)
 #pragma unroll
-      for (int n = 0; n < kNT; ++n)
+      for (int m = 0; m < kMT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[h][n][i] = 0.f;
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[h][m][n][i] = 0.f;
     __syncthreads();
 
-    const int g = lane >> 2, t = lane & 3, r0 = warp * 16 + g;
+    const int g = lane >> 2, t = lane & 3;
+    const int r0 = (kMT == 1 ? warp * 16 : (warp & 3) * 32) + g, kh = kMT == 1 ? 0 : warp >> 2;
     int slot = 0;
     uint32_t phase = 0;
     for (int i = 0; i < n_stages; ++i) {
@@ -162,38 +168,59 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
       const uint8_t* w = smem + slot * kStage;
       const uint8_t* xb = w + kWBytes;
       if (kW4) {
-        // lane t's codes are k = 32 t .. 32 t + 31, word j eight of them
-        const uint4 c0 = lds16(w + r0 * kRowCodeBytes + 16 * code_slot(r0, t));
-        const uint4 c1 = lds16(w + (r0 + 8) * kRowCodeBytes + 16 * code_slot(r0 + 8, t));
-        const uint8_t* sc = w + kTileCodeBytes + r0 * kRowScaleBytes + 2 * t;
-        uint32_t s0[2], s1[2];
-        expand_scales<kHalf>(*reinterpret_cast<const uint16_t*>(sc), s0[0], s0[1]);
-        expand_scales<kHalf>(*reinterpret_cast<const uint16_t*>(sc + 8 * kRowScaleBytes), s1[0], s1[1]);
-        const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+        // lane t's codes are k = 32 t .. 32 t + 31 in four words; a scale covers two of them
+        constexpr int kWords = 4 / kMT;
+        uint32_t word[2 * kMT][kWords], scale[2 * kMT][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int h = 0; h < 2 * kMT; ++h) {
+          const int r = r0 + 8 * h;
+          const uint8_t* c = w + r * kRowCodeBytes + 16 * code_slot(r, t);
+          const uint8_t* sc = w + kTileCodeBytes + r * kRowScaleBytes + 2 * t;
+          if constexpr (kMT == 1) {
+            const uint4 v = lds16(c);
+            word[h][0] = v.x, word[h][1] = v.y, word[h][2] = v.z, word[h][3] = v.w;
+            expand_scales<kHalf>(*reinterpret_cast<const uint16_t*>(sc), scale[h][0], scale[h][1]);
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(c + 8 * kh);
+            word[h][0] = v.x, word[h][1] = v.y;
+            if (h & 1)   // two rows' scales at a time
+              expand_scales<kHalf>(sc[kh - 8 * kRowScaleBytes] | (uint32_t)sc[kh] << 8, scale[h - 1][0], scale[h][0]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
           uint4 b[kNT];
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) b[n] = box_piece(xb + (t >> 1) * kNT * 1024, 8 * n + g, (t & 1) * 4 + j);
-          uint32_t lo[4], hi[4];
-          dequant_word<kHalf>(w0[j], s0[j >> 1], a.m16, a.m64, lo);
-          dequant_word<kHalf>(w1[j], s1[j >> 1], a.m16, a.m64, hi);
+          for (int n = 0; n < kNT; ++n)
+            b[n] = box_piece(xb + (t >> 1) * kNT * 1024, 8 * n + g, (t & 1) * 4 + kWords * kh + j);
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) {
-            mma16816<kHalf>(acc[0][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
-            mma16816<kHalf>(acc[kSets - 1][n], lo[2], hi[2], lo[3], hi[3], b[n].z, b[n].w);
+          for (int m = 0; m < kMT; ++m) {
+            uint32_t lo[4], hi[4];
+            dequant_word<kHalf>(word[2 * m][j], scale[2 * m][kMT == 1 ? j >> 1 : 0], a.m16, a.m64, lo);
+            dequant_word<kHalf>(word[2 * m + 1][j], scale[2 * m + 1][kMT == 1 ? j >> 1 : 0], a.m16, a.m64, hi);
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) {
+              mma16816<kHalf>(acc[0][m][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
+              mma16816<kHalf>(acc[kSets - 1][m][n], lo[2], hi[2], lo[3], hi[3], b[n].z, b[n].w);
+            }
           }
         }
       } else {
-        // lane t's pieces are k = 16 t .. 16 t + 15
+        // lane t's pieces are k = 16 t .. 16 t + 15, two of eight
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 lo = box_piece(w, r0, 2 * t + j), hi = box_piece(w, r0 + 8, 2 * t + j);
+        for (int jj = 0; jj < 2 / kMT; ++jj) {
+          const int j = kMT == 1 ? jj : kh;
+          uint4 b[kNT];
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) {
-            const uint4 b = box_piece(xb, 8 * n + g, 2 * t + j);
-            mma16816<kHalf>(acc[0][n], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
-            mma16816<kHalf>(acc[kSets - 1][n], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+          for (int n = 0; n < kNT; ++n) b[n] = box_piece(xb, 8 * n + g, 2 * t + j);
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) {
+            const uint4 lo = box_piece(w, r0 + 16 * m, 2 * t + j), hi = box_piece(w, r0 + 16 * m + 8, 2 * t + j);
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) {
+              mma16816<kHalf>(acc[0][m][n], lo.x, hi.x, lo.y, hi.y, b[n].x, b[n].y);
+              mma16816<kHalf>(acc[kSets - 1][m][n], lo.z, hi.z, lo.w, hi.w, b[n].z, b[n].w);
+            }
           }
         }
       }
@@ -204,20 +231,28 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
         phase ^= 1;
       }
     }
+    auto each_sum = [&](auto&& f) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = r0 + 8 * h;
-      // output of the row, and whether it is the up half of a gated one
-      const int o = !kGated ? row : kW4 ? (row >> 5) * 16 + (row & 15) : row & 63;
-      const int up = !kGated ? 0 : kW4 ? (row >> 4) & 1 : row >> 6;
-      const int owner = o / share, at = owner * width + up * share + o - owner * share;
+      for (int h = 0; h < 2 * kMT; ++h) {
+        const int row = r0 + 8 * h;
+        // output of the row, and whether it is the up half of a gated one
+        const int o = !kGated ? row : kW4 ? (row >> 5) * 16 + (row & 15) : row & 63;
+        const int up = !kGated ? 0 : kW4 ? (row >> 4) & 1 : row >> 6;
+        const int owner = o / share, at = owner * width + up * share + o - owner * share;
 #pragma unroll
-      for (int n = 0; n < kNT; ++n)
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int tok = 8 * n + 2 * t + i;
-          if (tok < toks) sums[tok * kPitch + at] = acc[0][n][2 * h + i] + (kSets > 1 ? acc[kSets - 1][n][2 * h + i] : 0.f);
-        }
+          for (int i = 0; i < 2; ++i) {
+            const int tok = 8 * n + 2 * t + i;
+            const float v = acc[0][h >> 1][n][2 * (h & 1) + i];
+            if (tok < toks) f(sums[tok * kPitch + at], kSets > 1 ? v + acc[kSets - 1][h >> 1][n][2 * (h & 1) + i] : v);
+          }
+      }
+    };
+    if (kh == 0) each_sum([](float& s, float v) { s = v; });
+    if (kMT > 1) {   // the second half of k, once the first is there
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+      if (kh == 1) each_sum([](float& s, float v) { s += v; });
     }
   }
   if (!ok) give_up(a.error_flag);

@@ -24,14 +24,15 @@ int check_ffn(int tokens, int hidden, int inter) {
 }
 
 // How a forward product runs: few tokens stream the weights; else the cheaper side for the weights by
-// the sizes' estimates (64 tokens of the large layer: 25 against 38 us with the weights as rows),
-// tokens as rows where the pre-activations are kept.
-int (*forward_product(int t, int n, int k, int mode, bool keep))(const DenseGemm&, cudaStream_t) {
-  if (t <= kFewTokens) return launch_few_dense;
-  return !keep && swap_dense_cost(t, n, k) < dense_cost(t, n, k, mode, true) ? launch_swap_dense : launch_dense_gemm;
+// the sizes' estimates (64 x 7168 x 2048 block: 25 us with the weights as the MMA's rows, 38 as its
+// columns). It depends on the sizes alone, so a forward pass has the same bits whether it keeps its
+// pre-activations or not.
+int (*forward_product(int t, int n, int k, int mode))(const DenseGemm&, cudaStream_t) {
+  if (streams_dense(t, n, k)) return launch_few_dense;
+  return swap_dense_cost(t, n, k) < dense_cost(t, n, k, mode, true) ? launch_swap_dense : launch_dense_gemm;
 }
 size_t forward_scratch(int t, int n, int k, int mode) {
-  if (t <= kFewTokens) return 0;
+  if (streams_dense(t, n, k)) return 0;
   const size_t a = dense_scratch_bytes(t, n, k, mode, true), b = swap_dense_scratch_bytes(t, n, k);
   return a > b ? a : b;
 }
@@ -105,7 +106,7 @@ extern "C" int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int
   g.out = ws + l.h, g.ldo = inter;
   g.ab = ab;
   const cudaStream_t st = (cudaStream_t)stream;
-  if ((rc = forward_product(g.m, g.n, g.k, g.mode, ab != nullptr)(g, st))) return rc;
+  if ((rc = forward_product(g.m, g.n, g.k, g.mode)(g, st))) return rc;
   g.a = {ws + l.h, inter, true};
   g.b = {w2, ld2, true};
   g.n = hidden, g.k = inter;
@@ -113,7 +114,7 @@ extern "C" int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int
   g.out = out, g.ldo = hidden;
   g.ab = nullptr;
   g.add = add, g.ld_add = ld_add;
-  return forward_product(g.m, g.n, g.k, g.mode, false)(g, st);
+  return forward_product(g.m, g.n, g.k, g.mode)(g, st);
 }
 
 extern "C" int muse_moe_ffn_backward(const void* dy, long long ldy, const void* x, long long ldx, int dtype, int tokens,

@@ -385,6 +385,17 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
         tmem_ld_frag(acc + c + (16u << 16), hi);
         ptx::tmem_wait_ld();
         const int tok0 = t.tok0 + c, toks = min(32, n_tok - c);
+        if (!kW4 && kGated && a.l.ab && outs > 0) {   // keep the pre-activations: eight outputs of a token at a time
+          const int g = lane >> 2;
+          float* to = a.l.ab + (size_t)tok0 * 2 * a.l.n_out + o0 + g;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int tok = 8 * (j >> 2) + 2 * (lane & 3) + (j & 1), up = j & 2 ? a.l.n_out : 0;
+            if (tok >= toks) continue;
+            if (g < outs) to[(size_t)tok * 2 * a.l.n_out + up] = lo[j];
+            if (g + 8 < outs) to[(size_t)tok * 2 * a.l.n_out + up + 8] = hi[j];
+          }
+        }
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -470,6 +481,10 @@ __global__ void __launch_bounds__(256) swap_reduce(const Args a) {
     for (int k = 0; k < a.p.splits; ++k) {
       s += __ldcg(p + k * plane);
       if (kGated) u += __ldcg(p + k * plane + kGroup);
+    }
+    if (!kW4 && kGated && a.l.ab) {
+      a.l.ab[(size_t)tok * 2 * a.l.n_out + o] = s;
+      a.l.ab[(size_t)tok * 2 * a.l.n_out + a.l.n_out + o] = u;
     }
     float y = s * gs;
     if (kGated) y = silu_f(y) * (u * gs);
@@ -597,6 +612,7 @@ int launch_swap_dense(const DenseGemm& g, cudaStream_t st) {
   l.tokens = g.m;
   l.cols = g.k;
   l.n_out = gated ? g.n / 2 : g.n;
+  l.ab = gated ? g.ab : nullptr;
   l.padded_rows = padded_rows_of(g);
   CUtensorMap mw;
   const int rc = gated ? make_gated_map(&mw, g.b, l.n_out, g.k, g.dtype)

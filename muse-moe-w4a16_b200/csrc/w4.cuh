@@ -20,6 +20,7 @@ struct LinearArgs {
   long long ld_add;
   uint16_t* out;
   long long ldo;
+  float* ab;                 // gated 16-bit weights: fp32 pre-activations to keep, [tokens, 2 n_out], or null
   int tokens, cols, n_out;   // n_out: columns of y
   int k_chunks;              // 128-code chunks of K
   int padded_rows;           // weight rows, padded to 128

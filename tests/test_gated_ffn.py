@@ -70,7 +70,8 @@ def test_entries_refuse_before_any_launch(pkg):
 
 SIZES = [(1, 8, 8), (1, 128, 64), (2, 72, 200), (7, 264, 136), (8, 1024, 512), (9, 64, 1032), (16, 2048, 768),
          (17, 200, 72), (31, 512, 264), (33, 1000, 128), (64, 128, 1000), (100, 640, 384), (128, 264, 520),
-         (129, 1032, 64), (255, 136, 136), (256, 512, 512), (257, 768, 328), (509, 520, 1288), (1025, 256, 320)]
+         (129, 1032, 64), (255, 136, 136), (256, 512, 512), (257, 768, 328), (509, 520, 1288), (1025, 256, 320),
+         (20, 4104, 2056), (32, 3080, 1368), (40, 8, 8), (600, 2056, 24), (2100, 72, 520)]
 
 
 @gpu

@@ -85,7 +85,8 @@ def test_parity(pkg, T, N, K, gated, add, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("T,N,K,gated", [(513, 1001, 1008, False), (1000, 1288, 2048, True), (2049, 640, 528, False)])
+@pytest.mark.parametrize("T,N,K,gated", [(513, 1001, 1008, False), (1000, 1288, 2048, True), (2049, 640, 528, False),
+                                         (2500, 66, 4112, True), (4096, 16, 16, False)])
 def test_parity_many_tokens(pkg, T, N, K, gated):
     run(pkg, T, N, K, gated, torch.bfloat16, True, seed=T)
 
