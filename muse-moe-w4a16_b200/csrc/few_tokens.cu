@@ -155,6 +155,7 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[h][m][n][i] = 0.f;
+    chain_wait();   // x comes after it, and the bounded waits below do not count the kernel before
     __syncthreads();
 
     const int g = lane >> 2, t = lane & 3;

@@ -241,6 +241,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
     }
   } else if (warp == 1) {
     if (rank == 0 && ptx::elect_one()) {
+      chain_wait();   // B comes after it: the bounded waits do not count the kernel before
       Pos s;
       int it = 0;
       for (int w = pair; w < total && ok; w += pairs, ++it) {
@@ -300,6 +301,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
       }
     }
   } else if (kW4 && warp >= kDeqWarp0 && warp < kEpiWarp0<kW4>) {
+    chain_wait();
     // four groups of four warps: group (p, h) takes half h of every second chunk
     const int h = ((warp - kDeqWarp0) >> 2) & 1;      // 64-k half of the chunk
     const int r = (warp & 3) * 32 + lane;             // weight row of the tile

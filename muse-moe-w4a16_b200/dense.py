@@ -57,6 +57,15 @@ def _same(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) 
         raise _bad(f"{name} is {t.dtype}, x {dtype}")
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the byte ranges of two tensors' elements meet."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _rows(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
     """`t` [..., width] as 16-byte aligned rows and their stride: in place where its strides
     allow it, else a contiguous copy."""
@@ -114,7 +123,8 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] times a prepared NVFP4 matrix: [..., N], or silu(gate) * up [..., N/2] for a gated
     one, plus `add` (same shape) if given. x is bf16 or fp16, and so are add and the result; any
-    number of rows. Sums in fp32, one rounding. Inference only: it has no gradient."""
+    number of rows. Sums in fp32, one rounding. `out` receives the result if given; it may be `add`
+    itself. Inference only: it has no gradient."""
     _require_cuda(x, "x")
     K, n_out, w, dev = state["cols"], state["n_out"], state["w"], x.device
     dtype = _DTYPES.get(x.dtype)
@@ -146,6 +156,9 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
         out = x.new_empty(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         raise _bad(f"out must be a contiguous {x.dtype} {tuple(shape)} on {dev}")
+    elif _overlap(out, x) or (add is not None and _overlap(out, add)
+                              and (add.data_ptr() != out.data_ptr() or not add.is_contiguous())):
+        raise _bad("out may be add itself, but overlaps no input otherwise")
     gated = 1 if state["gated"] else 0
     n = _linear_workspace(T, state["rows"], K, gated)
     ws = _scratch(n, dev) if n else None
@@ -222,8 +235,10 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, add: torch.T
     """The gated feed-forward block (silu(x Wg^T) * (x Wu^T)) W2^T (+ add), 16-bit weights.
 
     x [..., H], w13 [2I, H] (gate rows, then up rows, as the routed experts' w13), w2 [H, I], add of
-    x's shape; all bf16 or all fp16; H and I multiples of 8. Differentiable in every tensor. A
-    pass that needs gradients keeps the pre-activations in fp32 (8 T I bytes)."""
+    x's shape; all bf16 or all fp16; H and I multiples of 8. Sums in fp32; the inner activation and the
+    gradients of the pre-activations are rounded to the tensors' type (fp16 ones overflow past
+    65504). Differentiable once in every tensor; a pass that needs gradients keeps the
+    pre-activations in fp32 (8 T I bytes). Equal inputs give equal bits, with or without gradients."""
     _require_cuda(x, "x")
     dev = x.device
     if x.dtype not in _DTYPES:

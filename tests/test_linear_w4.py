@@ -124,6 +124,15 @@ def test_strides_shapes_and_out(pkg, T):
     got = pkg.linear_w4(odd.view(1, T, 512), state, add=add.view(1, T, 300), out=out[1:T + 1].view(1, T, 300))
     assert got.shape == (1, T, 300) and torch.equal(out[1:T + 1], y)
     assert (out[0] == 7).all() and (out[-1] == 7).all()
+    # out may be add itself, and overlaps nothing else
+    both = add.clone()
+    assert pkg.linear_w4(x, state, add=both, out=both) is both and torch.equal(both, y)
+    room = torch.empty((T + 1, 300), dtype=x.dtype, device=DEV)
+    room[:-1] = add
+    for bad in (lambda: pkg.linear_w4(x, state, add=room[:-1], out=room[1:]),
+                lambda: pkg.linear_w4(x, state, out=x.view(-1)[:T * 300].view(T, 300))):
+        with pytest.raises(pkg.MuseError):
+            bad()
     one = x[:1].expand(T, 512)
     assert torch.equal(pkg.linear_w4(one, state), pkg.linear_w4(one.contiguous(), state))
 
