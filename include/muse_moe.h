@@ -384,13 +384,10 @@ int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int
  * out[t, n] = gs * sum_k x[t, k] * e2m1[n, k] * e4m3[n, k/16] (+ add[t, n]), or with gated
  * out[t, i] = silu(gate) * up (+ add), [tokens, rows/2]. rows, cols, gated as at the prepare call.
  * x: 16-byte aligned, ldx a multiple of 8. fp32 sums over weights that are exact in 16 bits, one
- * rounding at the end. workspace: muse_moe_linear_workspace_size bytes (0 for a few tokens),
- * 16-byte aligned, needs no initialisation. No counterpart in the reference.
+ * rounding at the end. No counterpart in the reference.
  */
-int muse_moe_linear_workspace_size(int tokens, int rows, int cols, int gated, size_t* bytes);
 int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int rows, int cols, int gated,
-                       const uint8_t* wp, const float* w_gs, const void* add, long long ld_add, void* out, long long ldo, void* workspace, size_t workspace_bytes,
-                       muse_stream_t stream);
+                       const uint8_t* wp, const float* w_gs, const void* add, long long ld_add, void* out, long long ldo, muse_stream_t stream);
 
 /*
  * The gated feed-forward block with 16-bit weights w13 [2 * inter, hidden] (gate rows, then up

@@ -62,9 +62,7 @@ SIGNATURES: dict[str, tuple] = {
                                       _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "muse_moe_linear_prepared_size": (_I, [_I, _I, _I, _SIZE_P]),
     "muse_moe_prepare_linear": (_I, [_P, _P, _I, _I, _I, _P, _P]),
-    "muse_moe_linear_w4": (_I, [_P, _L, _I, _I, _I, _I, _I, _P, _P, _P, _L, _P, _L, _P,
-                                ctypes.c_size_t, _P]),
-    "muse_moe_linear_workspace_size": (_I, [_I, _I, _I, _I, _SIZE_P]),
+    "muse_moe_linear_w4": (_I, [_P, _L, _I, _I, _I, _I, _I, _P, _P, _P, _L, _P, _L, _P]),
     "muse_moe_ffn_workspace_size": (_I, [_I, _I, _I, _I, _SIZE_P]),
     "muse_moe_ffn_forward": (_I, [_P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _P, _P, ctypes.c_size_t, _P]),
     "muse_moe_ffn_backward": (_I, [_P, _L, _P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _P, _P,

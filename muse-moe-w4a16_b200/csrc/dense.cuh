@@ -63,7 +63,6 @@ int make_gated_map(CUtensorMap* map, const DenseOperand& o, int inter, int k, in
 // M side (swap_gemm.cu), and both forms' estimated times in SM clocks.
 double dense_cost(int m, int n, int k, int mode, bool b_k_major);
 double swap_dense_cost(int m, int n, int k);
-size_t swap_dense_scratch_bytes(int m, int n, int k);
 int launch_swap_dense(const DenseGemm& g, cudaStream_t stream);
 
 // ---- 16-bit conversions shared by the dense kernels

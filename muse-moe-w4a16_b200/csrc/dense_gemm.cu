@@ -393,7 +393,7 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
   __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
-  cluster_sync();  // the pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
+  cluster_sync_relaxed();  // the pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
   ptx::tc_fence_after();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");

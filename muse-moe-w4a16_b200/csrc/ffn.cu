@@ -32,9 +32,8 @@ int (*forward_product(int t, int n, int k, int mode))(const DenseGemm&, cudaStre
   return swap_dense_cost(t, n, k) < dense_cost(t, n, k, mode, true) ? launch_swap_dense : launch_dense_gemm;
 }
 size_t forward_scratch(int t, int n, int k, int mode) {
-  if (streams_dense(t, n, k)) return 0;
-  const size_t a = dense_scratch_bytes(t, n, k, mode, true), b = swap_dense_scratch_bytes(t, n, k);
-  return a > b ? a : b;
+  if (forward_product(t, n, k, mode) != launch_dense_gemm) return 0;
+  return dense_scratch_bytes(t, n, k, mode, true);
 }
 
 size_t up(size_t v) { return align_up(v, kAlign); }

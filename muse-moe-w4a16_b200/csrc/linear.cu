@@ -84,21 +84,9 @@ extern "C" int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, in
   return last_launch_status();
 }
 
-extern "C" int muse_moe_linear_workspace_size(int tokens, int rows, int cols, int gated, size_t* bytes) {
-  if (!bytes) return MUSE_ERR_INVALID_ARGUMENT;
-  const int rc = check_linear(rows, cols, gated);
-  if (rc) return rc;
-  if (tokens < 0) return MUSE_ERR_INVALID_ARGUMENT;
-  *bytes = tokens <= kFewTokens
-               ? 0
-               : linear_gemm_scratch_bytes(tokens, padded_rows_of(rows, gated), padded(cols, kChunkK) / kChunkK);
-  return MUSE_OK;
-}
-
 extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int rows, int cols, int gated,
                                   const uint8_t* wp, const float* w_gs, const void* add,
-                                  long long ld_add, void* out, long long ldo, void* workspace,
-                                  size_t workspace_bytes, muse_stream_t stream) {
+                                  long long ld_add, void* out, long long ldo, muse_stream_t stream) {
   int rc = check_linear(rows, cols, gated);
   if (rc) return rc;
   const int n_out = gated ? rows / 2 : rows;
@@ -124,12 +112,8 @@ extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int t
   a.k_chunks = padded(cols, kChunkK) / kChunkK;
   a.padded_rows = padded_rows_of(rows, gated);
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool few = tokens <= kFewTokens;
-  const size_t scratch = few ? 0 : linear_gemm_scratch_bytes(tokens, a.padded_rows, a.k_chunks);
-  if (scratch > 0 && (!workspace || misaligned(workspace, 16))) return MUSE_ERR_INVALID_ARGUMENT;
-  if (workspace_bytes < scratch) return MUSE_ERR_WORKSPACE_TOO_SMALL;
   int* flag = nullptr;
   if ((rc = device_status_ptr(&flag))) return rc;
-  if (few) return launch_few_w4(a, dtype, gated, flag, st);
-  return launch_linear_gemm(a, dtype, gated, static_cast<float*>(workspace), flag, st);
+  if (tokens <= kFewTokens) return launch_few_w4(a, dtype, gated, flag, st);
+  return launch_linear_gemm(a, dtype, gated, flag, st);
 }

@@ -16,6 +16,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// As cluster_sync, without ordering memory: before a CTA's shared and tensor memory go. (A release
+// would wait ~1000 clocks for the outputs' stores.)
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
+}
 // Address of the same shared-memory object in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
   uint32_t r;
@@ -49,12 +54,13 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-// Arrive on `bar` of both CTAs once this thread's MMAs so far have completed.
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+// Arrive on `bar` of both CTAs of the pair (`mask`: their bits in the cluster) once this thread's MMAs
+// so far have completed.
+__device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t mask = 3) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           ptx::smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"((uint16_t)mask)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {

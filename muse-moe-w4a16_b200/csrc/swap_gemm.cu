@@ -14,7 +14,10 @@
 // and turns them over (rows are weight rows, y's rows are tokens) with transposed matrix stores
 // into shared memory, so that global stores run along y's rows. Gated tiles hold gate and up rows
 // of an output in one thread's fragments.
-// With fewer tiles than pairs K is split; a second kernel adds the fp32 partials in split order.
+// With fewer tiles than pairs K is split over the pairs of a cluster (up to four). Each pair owns every
+// splits-th 32-token chunk of the tile's outputs and receives the other pairs' accumulators of it,
+// as fragments, through distributed shared memory (their rings are done by then): the owner adds
+// them to its own in split order and finishes the chunk. One launch, no scratch memory.
 // Bound by weight bytes (NVFP4: and the dequantisation) for tens of tokens, by the tensor pipe for
 // hundreds.
 #undef MUSE_TRACE  // these kernels record no stamps
@@ -57,26 +60,23 @@ struct Args {
   uint32_t idesc;
   uint32_t b_bytes;    // one CTA's B bytes per stage
   int out_vec, add_vec;  // rows of out / add are 16-byte aligned
-  float* partials;     // null: write the outputs
   int* error_flag;
 };
 
 struct Tile {
-  int m_tile, tok0, c0, c1, split;
+  int m_tile, tok0, c0, c1;
 };
-// Work item -> tile: splits innermost, then eight row tiles per token tile.
-__device__ __forceinline__ Tile tile_of(const GemmPlan& p, int w, uint32_t rank) {
+// Tile `idx` (eight row tiles per token tile) as CTA `rank` of pair `split` sees it.
+__device__ __forceinline__ Tile tile_of(const GemmPlan& p, int idx, uint32_t rank, int split) {
   constexpr int kGroup = 8;
   Tile t;
-  const int idx = w / p.splits;
-  t.split = w - idx * p.splits;
   const int group = idx / (kGroup * p.tiles_n);
   const int first = group * kGroup;
   const int rows = min(kGroup, p.tiles_m - first);
   const int r = idx - group * kGroup * p.tiles_n;
   t.m_tile = 2 * (first + r % rows) + (int)rank;
   t.tok0 = r / rows * p.bn;
-  t.c0 = t.split * p.units_per_split;
+  t.c0 = split * p.units_per_split;
   t.c1 = min(p.units, t.c0 + p.units_per_split);
   return t;
 }
@@ -184,9 +184,12 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   uint8_t* patches = codes + (kW4 ? kCodes * kCodeBytes : 0);
   Ctl& ctl = *reinterpret_cast<Ctl*>(patches + 4 * kPatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int total = a.p.tiles_m * a.p.tiles_n * a.p.splits;
+  // a cluster is the `splits` pairs of one tile at a time; `pair` counts clusters
+  const int splits = a.p.splits;
+  const uint32_t cta = cluster_rank(), rank = cta & 1, leader = cta & ~1u, mask = 3u << leader;
+  const int split = (int)(cta >> 1);
+  const int pair = blockIdx.x / (2 * splits), pairs = gridDim.x / (2 * splits);
+  const int total = a.p.tiles_m * a.p.tiles_n;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stages; ++s) {
@@ -218,12 +221,116 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   chain_release();
 
   bool ok = true;
+  // ---- epilogue of a tile: this pair's chunks of 32 tokens (all of them unless K is split)
+  constexpr int dtype = kHalf ? kFp16 : kBf16;
+  constexpr int kOut = kGated ? 16 : 32;                  // outputs of an epilogue warp
+  using Io = PatchIo<kOut>;
+  const int quarter = warp & 3, epi = warp - kEpiWarp0<kW4>, step = 32 * splits;
+  const int chunks = (a.p.bn / 32 + splits - 1) / splits; // most chunks of one owner
+  // another pair's fragments of this pair's chunk `i` (of pair `from`, without the owner itself)
+  auto received = [&](uint8_t* base, int from, int i) { return base + (((from * chunks + i) * 4 + epi) << 12) + lane * 16; };
+  uint4 ahead[Io::kPieces];                               // the next patch's addend
+  auto first_addend = [&](const Tile& t) {
+    const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
+    const int outs = min(kOut, a.l.n_out - o0), n_tok = min(a.p.bn, a.l.tokens - t.tok0);
+    if (a.l.add && outs > 0 && 32 * split < n_tok)
+      Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, t.tok0 + 32 * split, min(32, n_tok - 32 * split), outs, a.add_vec);
+  };
+  auto tile_epilogue = [&](const Tile& t, int buf) {
+    const uint32_t acc = tmem + ((uint32_t)quarter << 21) + buf * kMaxBn;
+    const float gs = kW4 ? __ldg(a.l.gs) * kUnscale<kHalf> : 1.f;
+    uint8_t* patch = patches + epi * kPatch;
+    const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
+    const int outs = min(kOut, a.l.n_out - o0);
+    const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
+    const bool adds = a.l.add && outs > 0;
+    for (int c = 32 * split; c < n_tok && t.m_tile * kTileM < a.l.padded_rows; c += step) {
+      // fragments of rows 0-15 and 16-31 of the warp's quarter (gated: gate and up of the same
+      // outputs), through a transposed patch [token][output] so that stores run along outputs
+      float lo[16], hi[16];
+      tmem_ld_frag(acc + c, lo);
+      tmem_ld_frag(acc + c + (16u << 16), hi);
+      ptx::tmem_wait_ld();
+      for (int from = 0; from < splits - 1; ++from) {
+        const uint8_t* v = received(smem, from, c / step);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(v + i * 512), y = *reinterpret_cast<const float4*>(v + (i + 4) * 512);
+          lo[4 * i] += x.x, lo[4 * i + 1] += x.y, lo[4 * i + 2] += x.z, lo[4 * i + 3] += x.w;
+          hi[4 * i] += y.x, hi[4 * i + 1] += y.y, hi[4 * i + 2] += y.z, hi[4 * i + 3] += y.w;
+        }
+      }
+      const int tok0 = t.tok0 + c, toks = min(32, n_tok - c);
+      if (!kW4 && kGated && a.l.ab && outs > 0) {   // keep the pre-activations: eight outputs of a token at a time
+        const int g = lane >> 2;
+        float* to = a.l.ab + (size_t)tok0 * 2 * a.l.n_out + o0 + g;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int tok = 8 * (j >> 2) + 2 * (lane & 3) + (j & 1), up = j & 2 ? a.l.n_out : 0;
+          if (tok >= toks) continue;
+          if (g < outs) to[(size_t)tok * 2 * a.l.n_out + up] = lo[j];
+          if (g + 8 < outs) to[(size_t)tok * 2 * a.l.n_out + up + 8] = hi[j];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * b + i;
+          if (!kGated) {
+            lo[j] *= gs;
+            hi[j] *= gs;
+          } else if (kW4) {          // rows 0-15 gate, 16-31 up
+            lo[j] = silu_f(lo[j] * gs) * (hi[j] * gs);
+          } else if (i < 2) {        // rows 0-7 gate, 8-15 up; 16-23 gate, 24-31 up
+            lo[j] = silu_f(lo[j]) * lo[j + 2];
+            lo[j + 2] = silu_f(hi[j]) * hi[j + 2];
+          }
+        }
+      __syncwarp();                                       // the patch's last readers are done
+      if (adds) {
+        Io::put(patch, lane, ahead);
+        if (c + step < n_tok)
+          Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, tok0 + step, min(32, n_tok - c - step), outs, a.add_vec);
+        __syncwarp();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t f[kGated ? 2 : 4];
+          ldmatrix2_t(patch_row(patch, 8 * b + (lane & 7), (lane >> 3) & 1), f[0], f[1]);
+          if (!kGated) ldmatrix2_t(patch_row(patch, 8 * b + (lane & 7), 2 + ((lane >> 3) & 1)), f[2], f[3]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 u = unpack16(dtype, f[i]);
+            lo[4 * b + 2 * i] += u.x;
+            lo[4 * b + 2 * i + 1] += u.y;
+            if (!kGated) {
+              const float2 w2 = unpack16(dtype, f[2 + i]);
+              hi[4 * b + 2 * i] += w2.x;
+              hi[4 * b + 2 * i + 1] += w2.y;
+            }
+          }
+        }
+        __syncwarp();
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        stmatrix2_t(patch_row(patch, 8 * b + (lane & 7), (lane >> 3) & 1), pack16(dtype, lo[4 * b], lo[4 * b + 1]),
+                    pack16(dtype, lo[4 * b + 2], lo[4 * b + 3]));
+        if (!kGated)
+          stmatrix2_t(patch_row(patch, 8 * b + (lane & 7), 2 + ((lane >> 3) & 1)),
+                      pack16(dtype, hi[4 * b], hi[4 * b + 1]), pack16(dtype, hi[4 * b + 2], hi[4 * b + 3]));
+      }
+      __syncwarp();
+      if (outs > 0) Io::store(patch, lane, a.l.out + o0, a.l.ldo, tok0, toks, outs, a.out_vec);
+    }
+  };
+
   if (warp == 0) {
     // Codes: written by prepare only, so they are fetched without waiting for the kernel before.
     if (kW4 && ptx::elect_one()) {
       Pos q;
       for (int w = pair; w < total && ok; w += pairs) {
-        const Tile t = tile_of(a.p, w, rank);
+        const Tile t = tile_of(a.p, w, rank, split);
         // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
         const int m = min(t.m_tile, a.l.padded_rows / kTileM - 1);
         for (int c = t.c0; c < t.c1; ++c) {
@@ -245,7 +352,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
       Pos s;
       int it = 0;
       for (int w = pair; w < total && ok; w += pairs, ++it) {
-        const Tile t = tile_of(a.p, w, rank);
+        const Tile t = tile_of(a.p, w, rank, split);
         const int buf = it & 1;
         if (!ptx::mbar_wait(&ctl.acc_empty[buf], ((it >> 1) & 1) ^ 1)) {
           ok = false;
@@ -264,23 +371,23 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, n > kUnit * t.c0 || j > 0);
-          commit_pair(&ctl.empty[s.slot]);
+          commit_pair(&ctl.empty[s.slot], mask);
           s.next(n_stages);
         }
-        commit_pair(&ctl.acc_full[buf]);
+        commit_pair(&ctl.acc_full[buf], mask);
       }
     }
   } else if (warp == 2) {
     if (ptx::elect_one()) {
       if (!kW4 && pair < total) {
         // 16-bit weights might have been written by the kernel before: only drawn into L2 ahead of it
-        const Tile t = tile_of(a.p, pair, rank);
+        const Tile t = tile_of(a.p, pair, rank, split);
         for (int n = t.c0; n < min(t.c1, t.c0 + n_stages); ++n) prefetch_weights<kGated>(&map_w, n * 64, t.m_tile);
       }
       chain_wait();
       Pos s;
       for (int w = pair; w < total && ok; w += pairs) {
-        const Tile t = tile_of(a.p, w, rank);
+        const Tile t = tile_of(a.p, w, rank, split);
         const int row = t.tok0 + (int)rank * (a.p.bn >> 1);
         for (int n = kUnit * t.c0; n < kUnit * t.c1; ++n) {
           if (!ptx::mbar_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
@@ -288,7 +395,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
             break;
           }
           if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], 2 * (a.b_bytes + (kW4 ? 0 : kABytes)));
-          const uint32_t dst = ptx::smem_u32(smem + s.slot * stage_bytes), bar = map_rank(&ctl.full[s.slot], 0);
+          const uint32_t dst = ptx::smem_u32(smem + s.slot * stage_bytes), bar = map_rank(&ctl.full[s.slot], leader);
           if (!kW4) load_weights<kGated>(dst, &map_w, n * 64, t.m_tile, bar);
           tma_pair(dst + kABytes, &map_x, n * 64, row, bar);
           s.next(n_stages);
@@ -309,7 +416,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
     Pos q, s;
     if (h) s.next(n_stages);
     for (int w = pair; w < total && ok; w += pairs) {
-      const Tile t = tile_of(a.p, w, rank);
+      const Tile t = tile_of(a.p, w, rank, split);
       for (int c = t.c0; c < t.c1; ++c, mine = !mine, q.next(kCodes), s.next(n_stages), s.next(n_stages)) {
         if (!mine) continue;
         if (!warp_wait(&ctl.code_full[q.slot], q.phase)) {
@@ -339,169 +446,80 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], 0));
+        if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], leader));
       }
     }
   } else if (warp >= kEpiWarp0<kW4>) {
     chain_wait();
-    const int quarter = warp & 3;
-    const uint32_t lane_base = tmem + ((uint32_t)quarter << 21);
-    constexpr int dtype = kHalf ? kFp16 : kBf16;
-    const float gs = kW4 ? __ldg(a.l.gs) * kUnscale<kHalf> : 1.f;
-    uint8_t* patch = patches + (warp - kEpiWarp0<kW4>) * kPatch;
-    int it = 0;
-    for (int w = pair; w < total; w += pairs, ++it) {
-      const Tile t = tile_of(a.p, w, rank);
-      const int buf = it & 1;
-      constexpr int kOut = kGated ? 16 : 32;              // outputs of the warp
-      using Io = PatchIo<kOut>;
-      const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
-      const int outs = min(kOut, a.l.n_out - o0);
-      const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
-      const bool adds = a.l.add && !a.partials && outs > 0;
-      uint4 ahead[Io::kPieces];                           // the next patch's addend
-      if (adds) Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, t.tok0, min(32, n_tok), outs, a.add_vec);
-      if (!warp_wait_sleep(&ctl.acc_full[buf], (it >> 1) & 1)) {
-        ok = false;
-        break;
-      }
-      ptx::tc_fence_after();
-      const uint32_t acc = lane_base + buf * kMaxBn;
-      const int row = t.m_tile * kTileM + quarter * 32 + lane;   // padded weight row
-      const bool tile_ok = t.m_tile * kTileM < a.l.padded_rows;
-      for (int c = 0; c < n_tok && tile_ok; c += 32) {
-        if (a.partials) {
-          float v[32];
-          tmem_ld32(acc + c, v);
-          ptx::tmem_wait_ld();
-          float* to = a.partials + ((size_t)t.split * a.l.tokens + t.tok0 + c) * a.l.padded_rows + row;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < n_tok) to[(size_t)j * a.l.padded_rows] = v[j];
-          continue;
+    if (splits == 1) {
+      int it = 0;
+      for (int w = pair; w < total && ok; w += pairs, ++it) {
+        const Tile t = tile_of(a.p, w, rank, split);
+        first_addend(t);
+        if (!warp_wait_sleep(&ctl.acc_full[it & 1], (it >> 1) & 1)) {
+          ok = false;
+          break;
         }
-        // fragments of rows 0-15 and 16-31 of the warp's quarter (gated: gate and up of the same
-        // outputs), through a transposed patch [token][output] so that stores run along outputs
-        float lo[16], hi[16];
-        tmem_ld_frag(acc + c, lo);
-        tmem_ld_frag(acc + c + (16u << 16), hi);
-        ptx::tmem_wait_ld();
-        const int tok0 = t.tok0 + c, toks = min(32, n_tok - c);
-        if (!kW4 && kGated && a.l.ab && outs > 0) {   // keep the pre-activations: eight outputs of a token at a time
-          const int g = lane >> 2;
-          float* to = a.l.ab + (size_t)tok0 * 2 * a.l.n_out + o0 + g;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int tok = 8 * (j >> 2) + 2 * (lane & 3) + (j & 1), up = j & 2 ? a.l.n_out : 0;
-            if (tok >= toks) continue;
-            if (g < outs) to[(size_t)tok * 2 * a.l.n_out + up] = lo[j];
-            if (g + 8 < outs) to[(size_t)tok * 2 * a.l.n_out + up + 8] = hi[j];
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = 4 * b + i;
-            if (!kGated) {
-              lo[j] *= gs;
-              hi[j] *= gs;
-            } else if (kW4) {          // rows 0-15 gate, 16-31 up
-              lo[j] = silu_f(lo[j] * gs) * (hi[j] * gs);
-            } else if (i < 2) {        // rows 0-7 gate, 8-15 up; 16-23 gate, 24-31 up
-              lo[j] = silu_f(lo[j]) * lo[j + 2];
-              lo[j + 2] = silu_f(hi[j]) * hi[j + 2];
-            }
-          }
-        __syncwarp();                                       // the patch's last readers are done
-        if (adds) {
-          Io::put(patch, lane, ahead);
-          if (c + 32 < n_tok)
-            Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, tok0 + 32, min(32, n_tok - c - 32), outs, a.add_vec);
-          __syncwarp();
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint32_t f[kGated ? 2 : 4];
-            ldmatrix2_t(patch_row(patch, 8 * b + (lane & 7), (lane >> 3) & 1), f[0], f[1]);
-            if (!kGated) ldmatrix2_t(patch_row(patch, 8 * b + (lane & 7), 2 + ((lane >> 3) & 1)), f[2], f[3]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float2 u = unpack16(dtype, f[i]);
-              lo[4 * b + 2 * i] += u.x;
-              lo[4 * b + 2 * i + 1] += u.y;
-              if (!kGated) {
-                const float2 w2 = unpack16(dtype, f[2 + i]);
-                hi[4 * b + 2 * i] += w2.x;
-                hi[4 * b + 2 * i + 1] += w2.y;
-              }
-            }
-          }
-          __syncwarp();
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          stmatrix2_t(patch_row(patch, 8 * b + (lane & 7), (lane >> 3) & 1), pack16(dtype, lo[4 * b], lo[4 * b + 1]),
-                      pack16(dtype, lo[4 * b + 2], lo[4 * b + 3]));
-          if (!kGated)
-            stmatrix2_t(patch_row(patch, 8 * b + (lane & 7), 2 + ((lane >> 3) & 1)),
-                        pack16(dtype, hi[4 * b], hi[4 * b + 1]), pack16(dtype, hi[4 * b + 2], hi[4 * b + 3]));
-        }
+        ptx::tc_fence_after();
+        tile_epilogue(t, it & 1);
+        ptx::tc_fence_before();
         __syncwarp();
-        if (outs > 0) Io::store(patch, lane, a.l.out + o0, a.l.ldo, tok0, toks, outs, a.out_vec);
+        if (lane == 0) arrive_cluster(map_rank(&ctl.acc_empty[it & 1], leader));
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_cluster(map_rank(&ctl.acc_empty[buf], 0));
+    } else {
+      first_addend(tile_of(a.p, pair, rank, split));
+      if (!warp_wait_sleep(&ctl.acc_full[0], 0)) ok = false;
+      ptx::tc_fence_after();
     }
   }
   if (!ok) give_up(a.error_flag);
   __syncwarp();
+  if (splits > 1) {
+    const Tile t = tile_of(a.p, pair, rank, split);
+    cluster_sync();   // every pair's MMAs are done, and with them the reads of the rings
+    if (warp >= kEpiWarp0<kW4>) {
+      const uint32_t acc = tmem + ((uint32_t)quarter << 21);
+      const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
+      for (int c = 0; c < n_tok; c += 32) {
+        const int owner = c / 32 % splits;
+        if (owner == split) continue;
+        float lo[16], hi[16];
+        tmem_ld_frag(acc + c, lo);
+        tmem_ld_frag(acc + c + (16u << 16), hi);
+        ptx::tmem_wait_ld();
+        const uint32_t to = map_rank(received(smem, split - (split > owner), c / step), 2 * owner + rank);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float* v = i < 4 ? lo + 4 * i : hi + 4 * (i - 4);
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + i * 512), "f"(v[0]), "f"(v[1]),
+                       "f"(v[2]), "f"(v[3])
+                       : "memory");
+        }
+      }
+    }
+    cluster_sync();
+    if (warp >= kEpiWarp0<kW4>) tile_epilogue(t, 0);
+    __syncwarp();
+  }
   ptx::tc_fence_before();
   __syncthreads();
-  cluster_sync();  // the pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
+  cluster_sync_relaxed();  // the pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
   ptx::tc_fence_after();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Sum of the splits' partials in split order, scale, gate and addend; one output per thread.
-template <bool kW4, bool kHalf, bool kGated>
-__global__ void __launch_bounds__(256) swap_reduce(const Args a) {
-  chain_release();
-  chain_wait();
-  constexpr int dtype = kHalf ? kFp16 : kBf16;
-  constexpr int kGroup = kW4 ? 16 : 8;   // gate rows in a row, then their up rows
-  const float gs = kW4 ? __ldg(a.l.gs) * kUnscale<kHalf> : 1.f;
-  const size_t plane = (size_t)a.l.tokens * a.l.padded_rows;
-  const size_t items = (size_t)a.l.tokens * a.l.n_out;
-  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < items; i += (size_t)gridDim.x * blockDim.x) {
-    const int tok = (int)(i / a.l.n_out), o = (int)(i - (size_t)tok * a.l.n_out);
-    const int row = kGated ? o / kGroup * 2 * kGroup + o % kGroup : o;
-    const float* p = a.partials + (size_t)tok * a.l.padded_rows + row;
-    float s = 0.f, u = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < a.p.splits; ++k) {
-      s += __ldcg(p + k * plane);
-      if (kGated) u += __ldcg(p + k * plane + kGroup);
-    }
-    if (!kW4 && kGated && a.l.ab) {
-      a.l.ab[(size_t)tok * 2 * a.l.n_out + o] = s;
-      a.l.ab[(size_t)tok * 2 * a.l.n_out + a.l.n_out + o] = u;
-    }
-    float y = s * gs;
-    if (kGated) y = silu_f(y) * (u * gs);
-    if (a.l.add) y += load16(dtype, a.l.add + (size_t)tok * a.l.ld_add + o);
-    a.l.out[(size_t)tok * a.l.ldo + o] = round16(dtype, y);
-  }
-}
-
 constexpr int kPairs = 74;  // 148 SMs, two to a pair
+
+// Clusters of one, two, three and four pairs that are resident together (SMs come in groups of 16 to 20).
+constexpr int kClusters[5] = {0, kPairs, 33, 22, 15};
 
 // Token tile and split of K from the sizes alone: the least estimated time in SM clocks. A 64-k
 // stage costs its MMAs (2 bn) or, NVFP4, the ring's latency over its depth (~2600 from a freed stage
 // over dequantisation, cluster arrival, MMA and commit to the next free one), 16 bits, its loads
-// (~60 B per clock and SM from L2); a tile's start and epilogue 2000 + 8 per token; a split the second
-// kernel's launch and the partials' way through L2 (~2 KB per clock over the chip).
+// (~60 B per clock and SM from L2), and never less than its four MMAs take to issue (~295); a tile's
+// start and epilogue 2000 + 8 per token; a split its exchange with two cluster barriers, which wait
+// for the slowest pair, 4500 + 8 per token.
 template <bool kW4>
 GemmPlan make_plan(int tokens, int padded_rows, int units, double* cost_out = nullptr) {
   constexpr int kUnit = kW4 ? 2 : 1;
@@ -517,13 +535,15 @@ GemmPlan make_plan(int tokens, int padded_rows, int units, double* cost_out = nu
     p.stages = kRingBytes<kW4> / (kABytes + bn * 64);
     if (p.stages > kMaxStages) p.stages = kMaxStages;
     double stage = kW4 ? 2600.0 / p.stages : (128 + bn / 2) * 128 / 60.0;
+    if (stage < 295) stage = 295;
     if (2.0 * bn > stage) stage = 2.0 * bn;
-    for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= kPairs && kUnit * units / s >= 4)); ++s) {
+    for (int s = 1; s <= 4 && (s == 1 || (tiles <= kClusters[s] && kUnit * units / s >= 4)); ++s) {
       p.units_per_split = (units + s - 1) / s;
-      p.splits = (units + p.units_per_split - 1) / p.units_per_split;
-      const double waves = (double)((tiles * p.splits + kPairs - 1) / kPairs);
+      if ((units + p.units_per_split - 1) / p.units_per_split != s) continue;   // a pair would have nothing to do
+      p.splits = s;
+      const double waves = (double)((tiles + kClusters[s] - 1) / kClusters[s]);
       double cost = waves * (kUnit * p.units_per_split * stage) + 2000 + 8.0 * bn;
-      if (p.splits > 1) cost += 4000 + 8.0 * tokens * padded_rows * p.splits / 2000;
+      if (s > 1) cost += 4500 + 8.0 * bn;
       if (best.bn == 0 || cost < best_cost) {
         best = p;
         best_cost = cost;
@@ -545,29 +565,25 @@ int launch(const CUtensorMap& mx, const CUtensorMap& mw, const Args& a, cudaStre
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) set[dev] = true;
   }
-  const long long total = (long long)a.p.tiles_m * a.p.tiles_n * a.p.splits;
-  const int pairs = total < kPairs ? (int)total : kPairs;
-  int rc = launch_chained(swap_gemm<kW4, kHalf, kGated>, dim3(2 * pairs), dim3(kThreads<kW4>), kSmem<kW4>, st, 2, mx, mw, a);
-  if (rc || !a.partials) return rc;
-  const size_t blocks = ((size_t)a.l.tokens * a.l.n_out + 255) / 256;
-  return launch_chained(swap_reduce<kW4, kHalf, kGated>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256),
-                        0, st, 1, a);
+  const int tiles = a.p.tiles_m * a.p.tiles_n;
+  const int clusters = a.p.splits > 1 || tiles < kPairs ? tiles : kPairs;
+  return launch_chained(swap_gemm<kW4, kHalf, kGated>, dim3(2 * a.p.splits * clusters), dim3(kThreads<kW4>), kSmem<kW4>, st,
+                        2 * a.p.splits, mx, mw, a);
 }
 
 template <bool kW4>
-int launch_any(const LinearArgs& l, const GemmPlan& p, const CUtensorMap& mw, int dtype, bool gated, float* partials,
-               int* error_flag, cudaStream_t st) {
+int launch_any(const LinearArgs& l, const GemmPlan& p, const CUtensorMap& mw, int dtype, bool gated, int* error_flag,
+               cudaStream_t st) {
   Args a{};
   a.l = l;
   a.p = p;
-  if ((long long)p.tiles_m * p.tiles_n * p.splits > 0x7FFFFFFFLL) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  if ((long long)p.tiles_m * p.tiles_n > (1 << 28)) return MUSE_ERR_UNSUPPORTED_SHAPE;
   const uint32_t type = dtype == kBf16 ? 1u : 0u;  // operand format: 0 f16, 1 bf16
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
   a.b_bytes = (uint32_t)p.bn / 2 * 128;
   auto vec = [](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
   a.out_vec = vec(l.out, l.ldo);
   a.add_vec = vec(l.add, l.ld_add);
-  a.partials = p.splits > 1 ? partials : nullptr;
   a.error_flag = error_flag;
   CUtensorMap mx;
   const int rc = make_operand_map(&mx, DenseOperand{l.x, l.ldx, true}, l.tokens, l.cols, dtype, p.bn / 2);
@@ -580,26 +596,14 @@ int padded_rows_of(const DenseGemm& g) { return (g.n + kTileM - 1) / kTileM * kT
 
 }  // namespace
 
-size_t linear_gemm_scratch_bytes(int tokens, int padded_rows, int k_chunks) {
-  const GemmPlan p = make_plan<true>(tokens, padded_rows, k_chunks);
-  return p.splits > 1 ? (size_t)4 * p.splits * tokens * padded_rows : 0;
-}
-
-int launch_linear_gemm(const LinearArgs& l, int dtype, bool gated, float* partials, int* error_flag, cudaStream_t st) {
-  return launch_any<true>(l, make_plan<true>(l.tokens, l.padded_rows, l.k_chunks), CUtensorMap{}, dtype, gated, partials,
-                          error_flag, st);
+int launch_linear_gemm(const LinearArgs& l, int dtype, bool gated, int* error_flag, cudaStream_t st) {
+  return launch_any<true>(l, make_plan<true>(l.tokens, l.padded_rows, l.k_chunks), CUtensorMap{}, dtype, gated, error_flag, st);
 }
 
 double swap_dense_cost(int m, int n, int k) {
   double cost;
   make_plan<false>(m, (n + kTileM - 1) / kTileM * kTileM, (k + 63) / 64, &cost);
   return cost;
-}
-
-size_t swap_dense_scratch_bytes(int m, int n, int k) {
-  const int rows = (n + kTileM - 1) / kTileM * kTileM;
-  const GemmPlan p = make_plan<false>(m, rows, (k + 63) / 64);
-  return p.splits > 1 ? (size_t)4 * p.splits * m * rows : 0;
 }
 
 int launch_swap_dense(const DenseGemm& g, cudaStream_t st) {
@@ -620,8 +624,7 @@ int launch_swap_dense(const DenseGemm& g, cudaStream_t st) {
   const int rc = gated ? make_gated_map(&mw, g.b, l.n_out, g.k, g.dtype)
                        : make_operand_map(&mw, g.b, g.n, g.k, g.dtype, kTileM);
   if (rc) return rc;
-  return launch_any<false>(l, make_plan<false>(g.m, l.padded_rows, (g.k + 63) / 64), mw, g.dtype, gated, g.partials,
-                           g.error_flag, st);
+  return launch_any<false>(l, make_plan<false>(g.m, l.padded_rows, (g.k + 63) / 64), mw, g.dtype, gated, g.error_flag, st);
 }
 
 }  // namespace muse

@@ -28,8 +28,7 @@ struct LinearArgs {
 };
 
 // The product for more than a few tokens.
-size_t linear_gemm_scratch_bytes(int tokens, int padded_rows, int k_chunks);
-int launch_linear_gemm(const LinearArgs& a, int dtype, bool gated, float* partials, int* error_flag, cudaStream_t st);
+int launch_linear_gemm(const LinearArgs& a, int dtype, bool gated, int* error_flag, cudaStream_t st);
 
 __device__ __forceinline__ uint32_t mul2_bf16(uint32_t a, uint32_t b) {
   uint32_t d;

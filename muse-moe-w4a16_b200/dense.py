@@ -112,13 +112,6 @@ def prepare_linear(weight: LinearWeights, gated: bool = False) -> dict:
             "rows": N, "cols": K, "gated": bool(gated), "n_out": N // 2 if gated else N}
 
 
-@functools.lru_cache(maxsize=4096)
-def _linear_workspace(tokens: int, rows: int, cols: int, gated: int) -> int:
-    n = ctypes.c_size_t(0)
-    _lib.call("muse_moe_linear_workspace_size", tokens, rows, cols, gated, ctypes.byref(n))
-    return n.value
-
-
 def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] times a prepared NVFP4 matrix: [..., N], or silu(gate) * up [..., N/2] for a gated
@@ -159,11 +152,8 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
     elif _overlap(out, x) or (add is not None and _overlap(out, add)
                               and (add.data_ptr() != out.data_ptr() or not add.is_contiguous())):
         raise _bad("out may be add itself, but overlaps no input otherwise")
-    gated = 1 if state["gated"] else 0
-    n = _linear_workspace(T, state["rows"], K, gated)
-    ws = _scratch(n, dev) if n else None
-    _call(dev.index, "muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, gated, w.data_ptr(),
-          state["w_gs"].data_ptr(), add_ptr, ld_add, out.data_ptr(), n_out, ws.data_ptr() if n else None, n)
+    _call(dev.index, "muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, 1 if state["gated"] else 0,
+          w.data_ptr(), state["w_gs"].data_ptr(), add_ptr, ld_add, out.data_ptr(), n_out)
     return out
 
 

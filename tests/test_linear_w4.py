@@ -44,16 +44,13 @@ def test_entry_refuses_before_any_launch(pkg):
     lib = pkg.load_library()
     call = lambda **k: lib.muse_moe_linear_w4(*[{**dict(  # noqa: E731
         x=256, ldx=64, dtype=0, tokens=2, rows=32, cols=64, gated=0, wp=256, gs=256, add=None, ld_add=0,
-        out=256, ldo=32, ws=256, bytes=1 << 30, stream=None), **k}[n] for n in ("x", "ldx", "dtype", "tokens", "rows", "cols", "gated", "wp",
-                                                        "gs", "add", "ld_add", "out", "ldo", "ws", "bytes", "stream")])
+        out=256, ldo=32, stream=None), **k}[n] for n in ("x", "ldx", "dtype", "tokens", "rows", "cols", "gated", "wp",
+                                                        "gs", "add", "ld_add", "out", "ldo", "stream")])
     assert call(tokens=0) == 0
     for bad in (dict(tokens=-1), dict(dtype=2), dict(x=None), dict(wp=None), dict(gs=None), dict(out=None),
                 dict(x=264), dict(ldx=68), dict(ldx=56), dict(ldo=31), dict(add=256, ld_add=31)):
         assert call(**bad) == -1, bad
     assert call(cols=40) == -2
-    # 40 tokens of a small matrix split K and need scratch
-    assert call(tokens=40, rows=128, cols=4096, ldx=4096, ldo=128, bytes=16) == -3
-    assert call(tokens=40, rows=128, cols=4096, ldx=4096, ldo=128, ws=None) == -1
 
 
 # ------------------------------------------------------------------ parity
