@@ -191,14 +191,29 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   const int pair = blockIdx.x / (2 * splits), pairs = gridDim.x / (2 * splits);
   const int total = a.p.tiles_m * a.p.tiles_n;
 
-  if (threadIdx.x == 0) {
+  // The first codes are fetched before anything else: they depend on no other CTA, and prepare alone
+  // writes them, so not on the kernel before either.
+  auto load_codes = [&](const Tile& t, int c, int slot) {
+    // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
+    const int m = min(t.m_tile, a.l.padded_rows / kTileM - 1);
+    ptx::mbar_arrive_expect_tx(&ctl.code_full[slot], kCodeBytes);
+    ptx::bulk_g2s(codes + slot * kCodeBytes, a.l.wq + ((size_t)m * a.p.units + c) * kLinearTileBytes, kCodeBytes,
+                  &ctl.code_full[slot]);
+  };
+  int early = 0;
+  if (kW4 && threadIdx.x == 0) {
+    for (int s = 0; s < kCodes; ++s) {
+      ptx::mbar_init(&ctl.code_full[s], 1);
+      ptx::mbar_init(&ctl.code_empty[s], 8);
+    }
+    ptx::fence_barrier_init();
+    const Tile t = tile_of(a.p, pair, rank, split);
+    for (; early < kCodes && t.c0 + early < t.c1; ++early) load_codes(t, t.c0 + early, early);
+  }
+  if (threadIdx.x == 64) {
     for (int s = 0; s < n_stages; ++s) {
       ptx::mbar_init(&ctl.full[s], kW4 ? 1 + 2 * 4 : 1);  // bytes announced by the leader; NVFP4's A by four warps of each CTA
       ptx::mbar_init(&ctl.empty[s], 1);
-    }
-    for (int s = 0; kW4 && s < kCodes; ++s) {
-      ptx::mbar_init(&ctl.code_full[s], 1);
-      ptx::mbar_init(&ctl.code_empty[s], 8);
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(&ctl.acc_full[b], 1);
@@ -326,23 +341,20 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   };
 
   if (warp == 0) {
-    // Codes: written by prepare only, so they are fetched without waiting for the kernel before.
-    if (kW4 && ptx::elect_one()) {
+    if (kW4 && lane == 0) {
       Pos q;
       for (int w = pair; w < total && ok; w += pairs) {
         const Tile t = tile_of(a.p, w, rank, split);
-        // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
-        const int m = min(t.m_tile, a.l.padded_rows / kTileM - 1);
-        for (int c = t.c0; c < t.c1; ++c) {
+        for (int c = t.c0; c < t.c1; ++c, q.next(kCodes)) {
+          if (early > 0) {   // already on its way
+            --early;
+            continue;
+          }
           if (!ptx::mbar_wait_sleep(&ctl.code_empty[q.slot], q.phase ^ 1)) {
             ok = false;
             break;
           }
-          uint8_t* dst = codes + q.slot * kCodeBytes;
-          const size_t tile = (size_t)m * a.p.units + c;
-          ptx::mbar_arrive_expect_tx(&ctl.code_full[q.slot], kCodeBytes);
-          ptx::bulk_g2s(dst, a.l.wq + tile * kLinearTileBytes, kLinearTileBytes, &ctl.code_full[q.slot]);
-          q.next(kCodes);
+          load_codes(t, c, q.slot);
         }
       }
     }
