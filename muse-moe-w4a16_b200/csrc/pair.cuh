@@ -54,6 +54,25 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
+// As mma_pair with A in tensor memory: each CTA's 128 rows, 16 k in eight columns of 16-bit pairs.
+__device__ __forceinline__ void mma_pair_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Store 32 consecutive 32-bit columns of this thread's lane.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
 // Arrive on `bar` of both CTAs of the pair (`mask`: their bits in the cluster) once this thread's MMAs
 // so far have completed.
 __device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t mask = 3) {
@@ -111,9 +130,11 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
 template <bool kMn>
 constexpr uint32_t kStepDesc = kMn ? 16 * 128 / 16 : 2;
 
-// A whole warp waits for a phase: one lane polls (every polling lane is an access of its own to the
-// barrier, and the others' would slow the arrivals), the rest wait for it.
+// A whole warp waits for a phase. A phase that is over already costs one test by all lanes (~100
+// clocks less than one lane's test and the word to the others); else one lane polls, so that the
+// polling does not crowd out the arrivals.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
   int ok = 1;
   if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait(bar, parity);
   ok = __shfl_sync(0xffffffffu, ok, 0);

@@ -7,9 +7,10 @@
 //   16-bit weights: by TMA. Gated: a view of w13 as [I / 8][gate, up][8] rows puts eight gate rows
 //   and the eight matching up rows next to one another, in one box.
 //   NVFP4: per 128-code chunk a CTA copies its 128 rows' codes and scales (one bulk copy of 9 KiB)
-//   into a six-deep ring; sixteen warps turn them into exact 16-bit weights in registers and write
-//   them as the K-major swizzled A operand (thread = weight row, one 128-byte row of 64 k each).
-//   Weights are dequantised once per 256 tokens, which fits under the 512 clocks of a stage's MMAs.
+//   into an eight-deep ring; sixteen warps turn them into exact 16-bit weights in registers (thread =
+//   weight row) and store them to tensor memory, from where the MMAs read A. Through shared memory,
+//   which carries B, the codes and its own 16 KiB twice, a stage took ~450 clocks at 64 tokens and
+//   ~630 at 256.
 // Accumulators are double buffered in tensor memory; the epilogue reads them as matrix fragments
 // and turns them over (rows are weight rows, y's rows are tokens) with transposed matrix stores
 // into shared memory, so that global stores run along y's rows. Gated tiles hold gate and up rows
@@ -30,11 +31,13 @@ namespace {
 
 constexpr int kMaxStages = 12;
 constexpr int kABytes = kTileM * 128;
-constexpr int kCodes = 6;                    // code ring: 128-code chunks of 9 KiB
+constexpr int kCodes = 8;                    // code ring: 128-code chunks of 9 KiB
 constexpr int kCodeBytes = kLinearTileBytes;
-// 64-k stages: A (16 KiB) and half of B (64 bytes a token).
-template <bool kW4> constexpr int kRingBytes = 5 * 2 * kABytes + (kW4 ? 0 : 3 * kABytes);
-constexpr int kMaxBn = 256;
+// 64-k stages in shared memory: half of B (64 bytes a token) and, 16-bit weights, A (16 KiB). NVFP4's A
+// takes 32 columns of tensor memory.
+template <bool kW4> constexpr int kRingBytes = kW4 ? 8 * kABytes : 13 * kABytes;
+template <bool kW4> constexpr int kStageA = kW4 ? 0 : kABytes;
+constexpr int kTmemCols = 512;
 constexpr int kPatch = 32 * 64;              // an epilogue warp's outputs of 32 tokens, 64 bytes each
 constexpr int kDeqWarp0 = 4;                 // warps 0-2: codes, MMA, TMA; then dequantisers; then the epilogue
 template <bool kW4> constexpr int kEpiWarp0 = kW4 ? 20 : 4;
@@ -51,7 +54,7 @@ constexpr size_t kSmem = 1024 + (size_t)kRingBytes<kW4> + (kW4 ? kCodes * kCodeB
 static_assert(kSmem<true> <= 232448 && kSmem<false> <= 232448, "shared memory of one CTA");
 
 struct GemmPlan {
-  int bn, stages, tiles_m, tiles_n, splits, units, units_per_split;  // units of K: 128 codes or 64 columns
+  int bn, accs, stages, tiles_m, tiles_n, splits, units, units_per_split;  // units of K: 128 codes or 64 columns
 };
 
 struct Args {
@@ -180,7 +183,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* codes = smem + kRingBytes<kW4>;
-  const int n_stages = a.p.stages, stage_bytes = kABytes + a.p.bn * 64;
+  const int n_stages = a.p.stages, stage_bytes = kStageA<kW4> + a.p.bn * 64;
   uint8_t* patches = codes + (kW4 ? kCodes * kCodeBytes : 0);
   Ctl& ctl = *reinterpret_cast<Ctl*>(patches + 4 * kPatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -233,6 +236,8 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   cluster_sync();
   ptx::tc_fence_after();
   const uint32_t tmem = ctl.tmem;
+  // tensor memory: one accumulator (two where a pair has several tiles), then NVFP4's A stages
+  const uint32_t a_cols = tmem + a.p.accs * a.p.bn;
   chain_release();
 
   bool ok = true;
@@ -252,7 +257,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
       Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, t.tok0 + 32 * split, min(32, n_tok - 32 * split), outs, a.add_vec);
   };
   auto tile_epilogue = [&](const Tile& t, int buf) {
-    const uint32_t acc = tmem + ((uint32_t)quarter << 21) + buf * kMaxBn;
+    const uint32_t acc = tmem + ((uint32_t)quarter << 21) + buf * a.p.bn;
     const float gs = kW4 ? __ldg(a.l.gs) * kUnscale<kHalf> : 1.f;
     uint8_t* patch = patches + epi * kPatch;
     const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
@@ -371,7 +376,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
           break;
         }
         ptx::tc_fence_after();
-        const uint32_t d = tmem + buf * kMaxBn;
+        const uint32_t d = tmem + buf * a.p.bn;
         for (int n = kUnit * t.c0; n < kUnit * t.c1; ++n) {
           if (!ptx::mbar_wait(&ctl.full[s.slot], s.phase)) {
             ok = false;
@@ -379,10 +384,15 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
           }
           ptx::tc_fence_after();
           const uint32_t sa = ptx::smem_u32(smem + s.slot * stage_bytes);
-          const uint64_t da = operand_desc<false>(sa), db = operand_desc<false>(sa + kABytes);
+          const uint64_t da = operand_desc<false>(sa), db = operand_desc<false>(sa + kStageA<kW4>);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, n > kUnit * t.c0 || j > 0);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t more = n > kUnit * t.c0 || j > 0;
+            if (kW4)
+              mma_pair_ts(d, a_cols + 32 * s.slot + 8 * j, db + j * kStepDesc<false>, a.idesc, more);
+            else
+              mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, more);
+          }
           commit_pair(&ctl.empty[s.slot], mask);
           s.next(n_stages);
         }
@@ -409,7 +419,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
           if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], 2 * (a.b_bytes + (kW4 ? 0 : kABytes)));
           const uint32_t dst = ptx::smem_u32(smem + s.slot * stage_bytes), bar = map_rank(&ctl.full[s.slot], leader);
           if (!kW4) load_weights<kGated>(dst, &map_w, n * 64, t.m_tile, bar);
-          tma_pair(dst + kABytes, &map_x, n * 64, row, bar);
+          tma_pair(dst + kStageA<kW4>, &map_x, n * 64, row, bar);
           s.next(n_stages);
         }
       }
@@ -421,45 +431,52 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
     }
   } else if (kW4 && warp >= kDeqWarp0 && warp < kEpiWarp0<kW4>) {
     chain_wait();
-    // four groups of four warps: group (p, h) takes half h of every second chunk
-    const int h = ((warp - kDeqWarp0) >> 2) & 1;      // 64-k half of the chunk
-    const int r = (warp & 3) * 32 + lane;             // weight row of the tile
-    bool mine = warp < kDeqWarp0 + 8;
+    // Four groups of four warps: group (p, h) takes half h of every second chunk, thread = weight row. The
+    // chunks of all tiles are one sequence here.
+    const int h = ((warp - kDeqWarp0) >> 2) & 1;
+    const int r = (warp & 3) * 32 + lane;
+    const Tile any = tile_of(a.p, pair, rank, split);
+    const int n = pair < total ? ((total - pair + pairs - 1) / pairs) * (any.c1 - any.c0) : 0;
+    int i = (warp - kDeqWarp0) >> 3;
     Pos q, s;
-    if (h) s.next(n_stages);
-    for (int w = pair; w < total && ok; w += pairs) {
-      const Tile t = tile_of(a.p, w, rank, split);
-      for (int c = t.c0; c < t.c1; ++c, mine = !mine, q.next(kCodes), s.next(n_stages), s.next(n_stages)) {
-        if (!mine) continue;
-        if (!warp_wait(&ctl.code_full[q.slot], q.phase)) {
-          ok = false;
-          break;
-        }
-        const uint8_t* src = codes + q.slot * kCodeBytes;
-        const uint4 c0 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h));
-        const uint4 c1 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h + 1));
-        const uint32_t sc = *reinterpret_cast<const uint32_t*>(src + kTileCodeBytes + r * kRowScaleBytes + 4 * h);
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&ctl.code_empty[q.slot]);
-        uint32_t scale[4];
-        expand_scales<kHalf>(sc & 0xFFFF, scale[0], scale[1]);
-        expand_scales<kHalf>(sc >> 16, scale[2], scale[3]);
-        if (!warp_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
-          ok = false;
-          break;
-        }
-        uint8_t* dst = smem + s.slot * stage_bytes + r * 128;
-        const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t v[4];
-          dequant_word<kHalf>(word[i], scale[i >> 1], a.l.m16, a.l.m64, v);
-          *reinterpret_cast<uint4*>(dst + ((i ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], leader));
+    for (int k = 0; k < i; ++k) q.next(kCodes);
+    for (int k = 0; k < 2 * i + h; ++k) s.next(n_stages);
+    uint4 c0, c1;
+    uint32_t sc;
+    auto fetch = [&] {   // this group's next codes and scales into registers
+      if (!warp_wait(&ctl.code_full[q.slot], q.phase)) ok = false;
+      const uint8_t* src = codes + q.slot * kCodeBytes;
+      c0 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h));
+      c1 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h + 1));
+      sc = *reinterpret_cast<const uint32_t*>(src + kTileCodeBytes + r * kRowScaleBytes + 4 * h);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&ctl.code_empty[q.slot]);
+      q.next(kCodes);
+      q.next(kCodes);
+    };
+    if (i < n) fetch();
+    for (; i < n && ok; i += 2) {
+      uint32_t scale[4];
+      expand_scales<kHalf>(sc & 0xFFFF, scale[0], scale[1]);
+      expand_scales<kHalf>(sc >> 16, scale[2], scale[3]);
+      if (!warp_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
+        ok = false;
+        break;
       }
+      ptx::tc_fence_after();   // the MMAs that read this stage before
+      const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      uint32_t v[32];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        dequant_word<kHalf>(word[k], scale[k >> 1], a.l.m16, a.l.m64, *reinterpret_cast<uint32_t(*)[4]>(v + 4 * k));
+      tmem_st32(a_cols + ((uint32_t)(warp & 3) << 21) + 32 * s.slot, v);
+      if (i + 2 < n) fetch();  // while the store is on its way
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], leader));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s.next(n_stages);
     }
   } else if (warp >= kEpiWarp0<kW4>) {
     chain_wait();
@@ -527,7 +544,7 @@ constexpr int kPairs = 74;  // 148 SMs, two to a pair
 constexpr int kClusters[5] = {0, kPairs, 33, 22, 15};
 
 // Token tile and split of K from the sizes alone: the least estimated time in SM clocks. A 64-k
-// stage costs its MMAs (2 bn) or, NVFP4, the ring's latency over its depth (~2600 from a freed stage
+// stage costs its MMAs (2 bn) or, NVFP4, the ring's latency over its depth (~1800 from a freed stage
 // over dequantisation, cluster arrival, MMA and commit to the next free one), 16 bits, its loads
 // (~60 B per clock and SM from L2), and never less than its four MMAs take to issue (~295); a tile's
 // start and epilogue 2000 + 8 per token; a split its exchange with two cluster barriers, which wait
@@ -544,15 +561,21 @@ GemmPlan make_plan(int tokens, int padded_rows, int units, double* cost_out = nu
     p.tiles_n = (tokens + bn - 1) / bn;
     p.units = units;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    p.stages = kRingBytes<kW4> / (kABytes + bn * 64);
-    if (p.stages > kMaxStages) p.stages = kMaxStages;
-    double stage = kW4 ? 2600.0 / p.stages : (128 + bn / 2) * 128 / 60.0;
-    if (stage < 295) stage = 295;
-    if (2.0 * bn > stage) stage = 2.0 * bn;
     for (int s = 1; s <= 4 && (s == 1 || (tiles <= kClusters[s] && kUnit * units / s >= 4)); ++s) {
       p.units_per_split = (units + s - 1) / s;
       if ((units + p.units_per_split - 1) / p.units_per_split != s) continue;   // a pair would have nothing to do
       p.splits = s;
+      p.stages = kRingBytes<kW4> / (kStageA<kW4> + bn * 64);
+      if (p.stages > kMaxStages) p.stages = kMaxStages;
+      p.accs = tiles <= kPairs || s > 1 ? 1 : 2;
+      if (kW4) {
+        const int cols = (kTmemCols - p.accs * bn) / 32;
+        if (cols < 4) continue;   // four dequantising groups must not lap the ring
+        if (p.stages > cols) p.stages = cols;
+      }
+      double stage = kW4 ? 1800.0 / p.stages : (128 + bn / 2) * 128 / 60.0;
+      if (stage < 295) stage = 295;
+      if (2.0 * bn > stage) stage = 2.0 * bn;
       const double waves = (double)((tiles + kClusters[s] - 1) / kClusters[s]);
       double cost = waves * (kUnit * p.units_per_split * stage) + 2000 + 8.0 * bn;
       if (s > 1) cost += 4500 + 8.0 * bn;
