@@ -54,14 +54,6 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-// As mma_pair with A in tensor memory: each CTA's 128 rows, 16 k in eight columns of 16-bit pairs.
-__device__ __forceinline__ void mma_pair_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
 // Store 32 consecutive 32-bit columns of this thread's lane.
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -129,6 +121,54 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
 // Descriptor step of 16 k (in 16-byte units).
 template <bool kMn>
 constexpr uint32_t kStepDesc = kMn ? 16 * 128 / 16 : 2;
+
+// What differs between a CTA on its own (kCtas = 1) and a pair (2): tensor-memory allocation, the
+// MMAs (A from shared or tensor memory), their commits, TMA boxes, and where barriers live: those
+// that a pair shares are its leader's. M is 128 per CTA.
+template <int kCtas> struct Group;
+#define MUSE_GROUP_OPS(G)                                                                                            \
+  static __device__ __forceinline__ void alloc(uint32_t* dst, uint32_t cols) {                                      \
+    asm volatile("tcgen05.alloc.cta_group::" G ".sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::smem_u32(dst)), \
+                 "r"(cols) : "memory");                                                                             \
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::" G ".sync.aligned;" ::: "memory");                    \
+  }                                                                                                                 \
+  static __device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t cols) {                                   \
+    asm volatile("tcgen05.dealloc.cta_group::" G ".sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");   \
+  }                                                                                                                 \
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {    \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                                 \
+                 "tcgen05.mma.cta_group::" G ".kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),       \
+                 "r"(idesc), "r"(acc) : "memory");                                                                  \
+  }                                                                                                                 \
+  /* A in tensor memory: each CTA's 128 rows, 16 k in eight columns of 16-bit pairs */                              \
+  static __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) { \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                                 \
+                 "tcgen05.mma.cta_group::" G ".kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),     \
+                 "r"(idesc), "r"(acc) : "memory");                                                                  \
+  }                                                                                                                 \
+  static __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) { \
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::" G ".shared::cluster.global.mbarrier::complete_tx::bytes"     \
+                 " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), \
+                 "r"(bar) : "memory");                                                                              \
+  }                                                                                                                 \
+  static __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c3, uint32_t bar) { \
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::" G ".shared::cluster.global.mbarrier::complete_tx::bytes"     \
+                 " [%0], [%1, {%2, %3, %3, %4}], [%5];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0),  \
+                 "r"(0), "r"(c3), "r"(bar) : "memory");                                                             \
+  }
+template <> struct Group<1> {
+  MUSE_GROUP_OPS("1")
+  static __device__ __forceinline__ void commit(uint64_t* bar, uint32_t) { ptx::mma_commit(bar); }
+  static __device__ __forceinline__ uint32_t shared_bar(uint64_t* bar, uint32_t) { return ptx::smem_u32(bar); }
+  static __device__ __forceinline__ void arrive(uint64_t* bar, uint32_t) { ptx::mbar_arrive(bar); }
+};
+template <> struct Group<2> {
+  MUSE_GROUP_OPS("2")
+  static __device__ __forceinline__ void commit(uint64_t* bar, uint32_t mask) { commit_pair(bar, mask); }
+  static __device__ __forceinline__ uint32_t shared_bar(uint64_t* bar, uint32_t leader) { return map_rank(bar, leader); }
+  static __device__ __forceinline__ void arrive(uint64_t* bar, uint32_t leader) { arrive_cluster(map_rank(bar, leader)); }
+};
+#undef MUSE_GROUP_OPS
 
 // A whole warp waits for a phase. A phase that is over already costs one test by all lanes (~100
 // clocks less than one lane's test and the word to the others); else one lane polls, so that the

@@ -1,9 +1,11 @@
-// y = x . W^T with the weight rows on the MMA's M side ("swap-AB"), on tcgen05 CTA pairs: the product
+// y = x . W^T with the weight rows on the MMA's M side ("swap-AB"), on tcgen05: the product
 // of a prepared NVFP4 weight with more than a few tokens, and the feed-forward block's forward
 // products of 16-bit weights where that beats tokens on the M side (dense_gemm.cu).
 //
-// 256 weight rows per pair are M and up to 256 tokens N, in steps of 32, so a batch of any size
-// wastes little. B is x by TMA, each CTA half of the tokens. A is
+// 128 weight rows of a CTA are M and up to 256 tokens N, in steps of 32, so a batch of any size wastes
+// little. From a certain size a pair of CTAs works on one tile of 256 rows (cta_group::2: B is read
+// once for both); below, single CTAs issue their MMAs in half the time (an MMA of a pair takes its
+// issuer ~75 to 100 clocks however small N is, one of a CTA ~44). B is x by TMA. A is
 //   16-bit weights: by TMA. Gated: a view of w13 as [I / 8][gate, up][8] rows puts eight gate rows
 //   and the eight matching up rows next to one another, in one box.
 //   NVFP4: per 128-code chunk a CTA copies its 128 rows' codes and scales (one bulk copy of 9 KiB)
@@ -15,9 +17,9 @@
 // and turns them over (rows are weight rows, y's rows are tokens) with transposed matrix stores
 // into shared memory, so that global stores run along y's rows. Gated tiles hold gate and up rows
 // of an output in one thread's fragments.
-// With fewer tiles than pairs K is split over the pairs of a cluster (up to four). Each pair owns every
-// splits-th 32-token chunk of the tile's outputs and receives the other pairs' accumulators of it,
-// as fragments, through distributed shared memory (their rings are done by then): the owner adds
+// With fewer tiles than groups K is split over the groups (CTAs or pairs) of a cluster of up to eight
+// CTAs. Each group owns every splits-th 32-token chunk of the tile's outputs and receives the others'
+// accumulators of it, as fragments, through distributed shared memory (the rings are done by then): the owner adds
 // them to its own in split order and finishes the chunk. One launch, no scratch memory.
 // Bound by weight bytes (NVFP4: and the dequantisation) for tens of tokens, by the tensor pipe for
 // hundreds.
@@ -33,7 +35,7 @@ constexpr int kMaxStages = 12;
 constexpr int kABytes = kTileM * 128;
 constexpr int kCodes = 8;                    // code ring: 128-code chunks of 9 KiB
 constexpr int kCodeBytes = kLinearTileBytes;
-// 64-k stages in shared memory: half of B (64 bytes a token) and, 16-bit weights, A (16 KiB). NVFP4's A
+// 64-k stages in shared memory: B (128 bytes a token; half the tokens in a pair) and, 16-bit weights, A (16 KiB). NVFP4's A
 // takes 32 columns of tensor memory.
 template <bool kW4> constexpr int kRingBytes = kW4 ? 8 * kABytes : 13 * kABytes;
 template <bool kW4> constexpr int kStageA = kW4 ? 0 : kABytes;
@@ -54,7 +56,7 @@ constexpr size_t kSmem = 1024 + (size_t)kRingBytes<kW4> + (kW4 ? kCodes * kCodeB
 static_assert(kSmem<true> <= 232448 && kSmem<false> <= 232448, "shared memory of one CTA");
 
 struct GemmPlan {
-  int bn, accs, stages, tiles_m, tiles_n, splits, units, units_per_split;  // units of K: 128 codes or 64 columns
+  int ctas, bn, accs, stages, tiles_m, tiles_n, splits, units, units_per_split;  // units of K: 128 codes or 64 columns
 };
 
 struct Args {
@@ -69,7 +71,8 @@ struct Args {
 struct Tile {
   int m_tile, tok0, c0, c1;
 };
-// Tile `idx` (eight row tiles per token tile) as CTA `rank` of pair `split` sees it.
+// Tile `idx` (eight row tiles per token tile) as CTA `rank` of group `split` sees it.
+template <int kCtas>
 __device__ __forceinline__ Tile tile_of(const GemmPlan& p, int idx, uint32_t rank, int split) {
   constexpr int kGroup = 8;
   Tile t;
@@ -77,7 +80,7 @@ __device__ __forceinline__ Tile tile_of(const GemmPlan& p, int idx, uint32_t ran
   const int first = group * kGroup;
   const int rows = min(kGroup, p.tiles_m - first);
   const int r = idx - group * kGroup * p.tiles_n;
-  t.m_tile = 2 * (first + r % rows) + (int)rank;
+  t.m_tile = kCtas * (first + r % rows) + (int)rank;
   t.tok0 = r / rows * p.bn;
   t.c0 = split * p.units_per_split;
   t.c1 = min(p.units, t.c0 + p.units_per_split);
@@ -94,20 +97,23 @@ struct Pos {
       phase ^= 1;
     }
   }
+  __device__ __forceinline__ void skip(int n, int size) {   // n <= size
+    slot += n;
+    if (slot >= size) {
+      slot -= size;
+      phase ^= 1;
+    }
+  }
 };
 
 // 128 weight rows x 64 k of tile m_tile (16-bit weights) into shared memory, or into L2. Gated: eight
 // groups of eight gate and eight up rows.
-template <bool kGated>
+template <int kCtas, bool kGated>
 __device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* map, int k, int m_tile, uint32_t bar) {
   if (kGated)
-    asm volatile(
-        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %3, %4}], [%5];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(k), "r"(0), "r"(m_tile * 8), "r"(bar)
-        : "memory");
+    Group<kCtas>::tma_4d(dst, map, k, m_tile * 8, bar);
   else
-    tma_pair(dst, map, k, m_tile * kTileM, bar);
+    Group<kCtas>::tma_2d(dst, map, k, m_tile * kTileM, bar);
 }
 template <bool kGated>
 __device__ __forceinline__ void prefetch_weights(const CUtensorMap* map, int k, int m_tile) {
@@ -176,22 +182,23 @@ struct PatchIo {
   }
 };
 
-template <bool kW4, bool kHalf, bool kGated>
+template <int kCtas, bool kW4, bool kHalf, bool kGated>
 __global__ void __launch_bounds__(kThreads<kW4>, 1)
 swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Args a) {
+  using G = Group<kCtas>;
   constexpr int kUnit = kW4 ? 2 : 1;   // stages of a unit
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* codes = smem + kRingBytes<kW4>;
-  const int n_stages = a.p.stages, stage_bytes = kStageA<kW4> + a.p.bn * 64;
+  const int n_stages = a.p.stages, stage_bytes = kStageA<kW4> + a.b_bytes;
   uint8_t* patches = codes + (kW4 ? kCodes * kCodeBytes : 0);
   Ctl& ctl = *reinterpret_cast<Ctl*>(patches + 4 * kPatch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a cluster is the `splits` pairs of one tile at a time; `pair` counts clusters
+  // a cluster is the `splits` groups of one tile at a time; `team` counts clusters
   const int splits = a.p.splits;
-  const uint32_t cta = cluster_rank(), rank = cta & 1, leader = cta & ~1u, mask = 3u << leader;
-  const int split = (int)(cta >> 1);
-  const int pair = blockIdx.x / (2 * splits), pairs = gridDim.x / (2 * splits);
+  const uint32_t cta = cluster_rank(), rank = cta % kCtas, leader = cta - rank, mask = 3u << leader;
+  const int split = (int)(cta / kCtas);
+  const int team = blockIdx.x / (kCtas * splits), teams = gridDim.x / (kCtas * splits);
   const int total = a.p.tiles_m * a.p.tiles_n;
 
   // The first codes are fetched before anything else: they depend on no other CTA, and prepare alone
@@ -207,33 +214,28 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   if (kW4 && threadIdx.x == 0) {
     for (int s = 0; s < kCodes; ++s) {
       ptx::mbar_init(&ctl.code_full[s], 1);
-      ptx::mbar_init(&ctl.code_empty[s], 8);
+      ptx::mbar_init(&ctl.code_empty[s], 4);
     }
     ptx::fence_barrier_init();
-    const Tile t = tile_of(a.p, pair, rank, split);
+    const Tile t = tile_of<kCtas>(a.p, team, rank, split);
     for (; early < kCodes && t.c0 + early < t.c1; ++early) load_codes(t, t.c0 + early, early);
   }
   if (threadIdx.x == 64) {
     for (int s = 0; s < n_stages; ++s) {
-      ptx::mbar_init(&ctl.full[s], kW4 ? 1 + 2 * 4 : 1);  // bytes announced by the leader; NVFP4's A by four warps of each CTA
+      ptx::mbar_init(&ctl.full[s], kW4 ? 1 + kCtas * 4 : 1);  // bytes announced by the leader; NVFP4's A by four warps of each CTA
       ptx::mbar_init(&ctl.empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(&ctl.acc_full[b], 1);
-      ptx::mbar_init(&ctl.acc_empty[b], 2 * 4);
+      ptx::mbar_init(&ctl.acc_empty[b], kCtas * 4);
     }
     ptx::fence_barrier_init();
     ptx::prefetch_tensormap(&map_x);
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::smem_u32(&ctl.tmem)),
-                 "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
+  if (warp == 1) G::alloc(&ctl.tmem, kTmemCols);
   ptx::tc_fence_before();
   __syncthreads();
-  cluster_sync();
+  if (kCtas * splits > 1) cluster_sync();
   ptx::tc_fence_after();
   const uint32_t tmem = ctl.tmem;
   // tensor memory: one accumulator (two where a pair has several tiles), then NVFP4's A stages
@@ -348,8 +350,8 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   if (warp == 0) {
     if (kW4 && lane == 0) {
       Pos q;
-      for (int w = pair; w < total && ok; w += pairs) {
-        const Tile t = tile_of(a.p, w, rank, split);
+      for (int w = team; w < total && ok; w += teams) {
+        const Tile t = tile_of<kCtas>(a.p, w, rank, split);
         for (int c = t.c0; c < t.c1; ++c, q.next(kCodes)) {
           if (early > 0) {   // already on its way
             --early;
@@ -368,8 +370,8 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
       chain_wait();   // B comes after it: the bounded waits do not count the kernel before
       Pos s;
       int it = 0;
-      for (int w = pair; w < total && ok; w += pairs, ++it) {
-        const Tile t = tile_of(a.p, w, rank, split);
+      for (int w = team; w < total && ok; w += teams, ++it) {
+        const Tile t = tile_of<kCtas>(a.p, w, rank, split);
         const int buf = it & 1;
         if (!ptx::mbar_wait(&ctl.acc_empty[buf], ((it >> 1) & 1) ^ 1)) {
           ok = false;
@@ -389,37 +391,37 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
           for (int j = 0; j < 4; ++j) {
             const uint32_t more = n > kUnit * t.c0 || j > 0;
             if (kW4)
-              mma_pair_ts(d, a_cols + 32 * s.slot + 8 * j, db + j * kStepDesc<false>, a.idesc, more);
+              G::mma_ts(d, a_cols + 32 * s.slot + 8 * j, db + j * kStepDesc<false>, a.idesc, more);
             else
-              mma_pair(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, more);
+              G::mma(d, da + j * kStepDesc<false>, db + j * kStepDesc<false>, a.idesc, more);
           }
-          commit_pair(&ctl.empty[s.slot], mask);
+          G::commit(&ctl.empty[s.slot], mask);
           s.next(n_stages);
         }
-        commit_pair(&ctl.acc_full[buf], mask);
+        G::commit(&ctl.acc_full[buf], mask);
       }
     }
   } else if (warp == 2) {
     if (ptx::elect_one()) {
-      if (!kW4 && pair < total) {
+      if (!kW4 && team < total) {
         // 16-bit weights might have been written by the kernel before: only drawn into L2 ahead of it
-        const Tile t = tile_of(a.p, pair, rank, split);
+        const Tile t = tile_of<kCtas>(a.p, team, rank, split);
         for (int n = t.c0; n < min(t.c1, t.c0 + n_stages); ++n) prefetch_weights<kGated>(&map_w, n * 64, t.m_tile);
       }
       chain_wait();
       Pos s;
-      for (int w = pair; w < total && ok; w += pairs) {
-        const Tile t = tile_of(a.p, w, rank, split);
-        const int row = t.tok0 + (int)rank * (a.p.bn >> 1);
+      for (int w = team; w < total && ok; w += teams) {
+        const Tile t = tile_of<kCtas>(a.p, w, rank, split);
+        const int row = t.tok0 + (int)rank * (a.p.bn / kCtas);
         for (int n = kUnit * t.c0; n < kUnit * t.c1; ++n) {
           if (!ptx::mbar_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
             ok = false;
             break;
           }
-          if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], 2 * (a.b_bytes + (kW4 ? 0 : kABytes)));
-          const uint32_t dst = ptx::smem_u32(smem + s.slot * stage_bytes), bar = map_rank(&ctl.full[s.slot], leader);
-          if (!kW4) load_weights<kGated>(dst, &map_w, n * 64, t.m_tile, bar);
-          tma_pair(dst + kStageA<kW4>, &map_x, n * 64, row, bar);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&ctl.full[s.slot], kCtas * stage_bytes);
+          const uint32_t dst = ptx::smem_u32(smem + s.slot * stage_bytes), bar = G::shared_bar(&ctl.full[s.slot], leader);
+          if (!kW4) load_weights<kCtas, kGated>(dst, &map_w, n * 64, t.m_tile, bar);
+          G::tma_2d(dst + kStageA<kW4>, &map_x, n * 64, row, bar);
           s.next(n_stages);
         }
       }
@@ -431,59 +433,62 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
     }
   } else if (kW4 && warp >= kDeqWarp0 && warp < kEpiWarp0<kW4>) {
     chain_wait();
-    // Four groups of four warps: group (p, h) takes half h of every second chunk, thread = weight row. The
-    // chunks of all tiles are one sequence here.
-    const int h = ((warp - kDeqWarp0) >> 2) & 1;
+    // Up to four groups of four warps take the chunks (of all tiles, one sequence here) in turn, thread =
+    // weight row. A group may only wait for a stage whose use before last is known to be over, as
+    // the phases of a barrier are told apart by parity alone: two stages a group fit the ring.
+    const int groups = min(4, n_stages / 2), group = (warp - kDeqWarp0) >> 2;
     const int r = (warp & 3) * 32 + lane;
-    const Tile any = tile_of(a.p, pair, rank, split);
-    const int n = pair < total ? ((total - pair + pairs - 1) / pairs) * (any.c1 - any.c0) : 0;
-    int i = (warp - kDeqWarp0) >> 3;
+    const Tile any = tile_of<kCtas>(a.p, team, rank, split);
+    const int n = team < total && group < groups ? ((total - team + teams - 1) / teams) * (any.c1 - any.c0) : 0;
     Pos q, s;
-    for (int k = 0; k < i; ++k) q.next(kCodes);
-    for (int k = 0; k < 2 * i + h; ++k) s.next(n_stages);
-    uint4 c0, c1;
-    uint32_t sc;
+    q.skip(group, kCodes);
+    s.skip(2 * group, n_stages);
+    uint4 code[4];
+    uint2 sc;
     auto fetch = [&] {   // this group's next codes and scales into registers
       if (!warp_wait(&ctl.code_full[q.slot], q.phase)) ok = false;
       const uint8_t* src = codes + q.slot * kCodeBytes;
-      c0 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h));
-      c1 = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, 2 * h + 1));
-      sc = *reinterpret_cast<const uint32_t*>(src + kTileCodeBytes + r * kRowScaleBytes + 4 * h);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) code[k] = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, k));
+      sc = *reinterpret_cast<const uint2*>(src + kTileCodeBytes + r * kRowScaleBytes);
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&ctl.code_empty[q.slot]);
-      q.next(kCodes);
-      q.next(kCodes);
+      q.skip(groups, kCodes);
     };
-    if (i < n) fetch();
-    for (; i < n && ok; i += 2) {
-      uint32_t scale[4];
-      expand_scales<kHalf>(sc & 0xFFFF, scale[0], scale[1]);
-      expand_scales<kHalf>(sc >> 16, scale[2], scale[3]);
-      if (!warp_wait(&ctl.empty[s.slot], s.phase ^ 1)) {
-        ok = false;
-        break;
-      }
-      ptx::tc_fence_after();   // the MMAs that read this stage before
-      const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-      uint32_t v[32];
+    if (group < n) fetch();
+    for (int i = group; i < n && ok; i += groups) {
+      Pos at = s;
+      int slots[2];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        dequant_word<kHalf>(word[k], scale[k >> 1], a.l.m16, a.l.m64, *reinterpret_cast<uint32_t(*)[4]>(v + 4 * k));
-      tmem_st32(a_cols + ((uint32_t)(warp & 3) << 21) + 32 * s.slot, v);
-      if (i + 2 < n) fetch();  // while the store is on its way
+      for (int h = 0; h < 2; ++h) {   // a stage is half of the chunk
+        const uint32_t sch = h ? sc.y : sc.x;
+        uint32_t scale[4], v[32];
+        expand_scales<kHalf>(sch & 0xFFFF, scale[0], scale[1]);
+        expand_scales<kHalf>(sch >> 16, scale[2], scale[3]);
+        if (!warp_wait(&ctl.empty[at.slot], at.phase ^ 1)) ok = false;   // (then it runs on over what is there)
+        ptx::tc_fence_after();   // the MMAs that read this stage before
+        const uint32_t word[8] = {code[2 * h].x,     code[2 * h].y,     code[2 * h].z,     code[2 * h].w,
+                                  code[2 * h + 1].x, code[2 * h + 1].y, code[2 * h + 1].z, code[2 * h + 1].w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          dequant_word<kHalf>(word[k], scale[k >> 1], a.l.m16, a.l.m64, *reinterpret_cast<uint32_t(*)[4]>(v + 4 * k));
+        tmem_st32(a_cols + ((uint32_t)(warp & 3) << 21) + 32 * at.slot, v);
+        slots[h] = at.slot;
+        at.next(n_stages);
+      }
+      if (i + groups < n) fetch();  // while the stores are on their way
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_cluster(map_rank(&ctl.full[s.slot], leader));
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s.next(n_stages);
+      if (lane < 2) G::arrive(&ctl.full[lane ? slots[1] : slots[0]], leader);
+      s.skip(2 * groups, n_stages);
     }
   } else if (warp >= kEpiWarp0<kW4>) {
     chain_wait();
     if (splits == 1) {
       int it = 0;
-      for (int w = pair; w < total && ok; w += pairs, ++it) {
-        const Tile t = tile_of(a.p, w, rank, split);
+      for (int w = team; w < total && ok; w += teams, ++it) {
+        const Tile t = tile_of<kCtas>(a.p, w, rank, split);
         first_addend(t);
         if (!warp_wait_sleep(&ctl.acc_full[it & 1], (it >> 1) & 1)) {
           ok = false;
@@ -493,10 +498,10 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
         tile_epilogue(t, it & 1);
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_cluster(map_rank(&ctl.acc_empty[it & 1], leader));
+        if (lane == 0) G::arrive(&ctl.acc_empty[it & 1], leader);
       }
     } else {
-      first_addend(tile_of(a.p, pair, rank, split));
+      first_addend(tile_of<kCtas>(a.p, team, rank, split));
       if (!warp_wait_sleep(&ctl.acc_full[0], 0)) ok = false;
       ptx::tc_fence_after();
     }
@@ -504,7 +509,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   if (!ok) give_up(a.error_flag);
   __syncwarp();
   if (splits > 1) {
-    const Tile t = tile_of(a.p, pair, rank, split);
+    const Tile t = tile_of<kCtas>(a.p, team, rank, split);
     cluster_sync();   // every pair's MMAs are done, and with them the reads of the rings
     if (warp >= kEpiWarp0<kW4>) {
       const uint32_t acc = tmem + ((uint32_t)quarter << 21);
@@ -516,7 +521,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
         tmem_ld_frag(acc + c, lo);
         tmem_ld_frag(acc + c + (16u << 16), hi);
         ptx::tmem_wait_ld();
-        const uint32_t to = map_rank(received(smem, split - (split > owner), c / step), 2 * owner + rank);
+        const uint32_t to = map_rank(received(smem, split - (split > owner), c / step), kCtas * owner + rank);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float* v = i < 4 ? lo + 4 * i : hi + 4 * (i - 4);
@@ -532,78 +537,95 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   }
   ptx::tc_fence_before();
   __syncthreads();
-  cluster_sync_relaxed();  // the pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
+  // a pair's MMAs read both CTAs' shared memory, commits write both CTAs' barriers
+  if (kCtas > 1) cluster_sync_relaxed();
   ptx::tc_fence_after();
-  if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 1) G::dealloc(tmem, kTmemCols);
 }
 
-constexpr int kPairs = 74;  // 148 SMs, two to a pair
+constexpr int kSms = 148;
 
-// Clusters of one, two, three and four pairs that are resident together (SMs come in groups of 16 to 20).
-constexpr int kClusters[5] = {0, kPairs, 33, 22, 15};
+// Clusters of this many CTAs that are resident together (SMs come in groups of 16 to 20).
+constexpr int clusters_of(int ctas) {
+  return ctas == 1 ? kSms : ctas == 2 ? kSms / 2 : ctas == 4 ? 33 : ctas == 6 ? 22 : ctas == 8 ? 15 : 0;
+}
 
-// Token tile and split of K from the sizes alone: the least estimated time in SM clocks. A 64-k
-// stage costs its MMAs (2 bn) or, NVFP4, the ring's latency over its depth (~1800 from a freed stage
-// over dequantisation, cluster arrival, MMA and commit to the next free one), 16 bits, its loads
-// (~60 B per clock and SM from L2), and never less than its four MMAs take to issue (~295); a tile's
-// start and epilogue 2000 + 8 per token; a split its exchange with two cluster barriers, which wait
-// for the slowest pair, 4500 + 8 per token.
+// Groups of one CTA or two, token tile and split of K from the sizes alone: the least estimated time in
+// SM clocks. A 64-k stage costs its MMAs (2 bn) or more: NVFP4 what dequantisation and MMAs together
+// measured (400 + 1.2 bn for a CTA, 380 + 0.86 bn for a pair, whose B is shared) or the ring's latency
+// over its depth (~2400 from a freed stage over dequantisation, arrival, MMA and commit to the next
+// free one); 16 bits its loads (~60 B per clock and SM from L2) and its MMAs' issue (~200, a pair's
+// ~295). A tile's start and epilogue take 2000 + 8 per token, a split's exchange with two cluster
+// barriers, which wait for the slowest group, 4500 + 8 per token.
 template <bool kW4>
 GemmPlan make_plan(int tokens, int padded_rows, int units, double* cost_out = nullptr) {
   constexpr int kUnit = kW4 ? 2 : 1;
   GemmPlan best{};
   double best_cost = 0;
-  for (int bn = 32; bn <= 256; bn += 32) {
-    GemmPlan p;
-    p.bn = bn;
-    p.tiles_m = (padded_rows + 255) / 256;
-    p.tiles_n = (tokens + bn - 1) / bn;
-    p.units = units;
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    for (int s = 1; s <= 4 && (s == 1 || (tiles <= kClusters[s] && kUnit * units / s >= 4)); ++s) {
-      p.units_per_split = (units + s - 1) / s;
-      if ((units + p.units_per_split - 1) / p.units_per_split != s) continue;   // a pair would have nothing to do
-      p.splits = s;
-      p.stages = kRingBytes<kW4> / (kStageA<kW4> + bn * 64);
-      if (p.stages > kMaxStages) p.stages = kMaxStages;
-      p.accs = tiles <= kPairs || s > 1 ? 1 : 2;
-      if (kW4) {
-        const int cols = (kTmemCols - p.accs * bn) / 32;
-        if (cols < 4) continue;   // four dequantising groups must not lap the ring
-        if (p.stages > cols) p.stages = cols;
-      }
-      double stage = kW4 ? 1800.0 / p.stages : (128 + bn / 2) * 128 / 60.0;
-      if (stage < 295) stage = 295;
-      if (2.0 * bn > stage) stage = 2.0 * bn;
-      const double waves = (double)((tiles + kClusters[s] - 1) / kClusters[s]);
-      double cost = waves * (kUnit * p.units_per_split * stage) + 2000 + 8.0 * bn;
-      if (s > 1) cost += 4500 + 8.0 * bn;
-      if (best.bn == 0 || cost < best_cost) {
-        best = p;
-        best_cost = cost;
+  for (int ctas = 1; ctas <= 2; ++ctas)
+    for (int bn = 32; bn <= 128 * ctas; bn += 32) {
+      GemmPlan p;
+      p.ctas = ctas;
+      p.bn = bn;
+      p.tiles_m = (padded_rows + kTileM * ctas - 1) / (kTileM * ctas);
+      p.tiles_n = (tokens + bn - 1) / bn;
+      p.units = units;
+      const long long tiles = (long long)p.tiles_m * p.tiles_n;
+      for (int s = 1; s * ctas <= 8; ++s) {
+        const int room = clusters_of(s * ctas);
+        if (room == 0 || (s > 1 && (tiles > room || kUnit * units / s < 4))) continue;
+        p.units_per_split = (units + s - 1) / s;
+        if ((units + p.units_per_split - 1) / p.units_per_split != s) continue;   // a group would have nothing to do
+        p.splits = s;
+        const int stage_bytes = kStageA<kW4> + bn / ctas * 128;
+        p.stages = kRingBytes<kW4> / stage_bytes;
+        if (p.stages > kMaxStages) p.stages = kMaxStages;
+        p.accs = tiles <= room || s > 1 ? 1 : 2;
+        if (kW4) {
+          const int cols = (kTmemCols - p.accs * bn) / 32;
+          if (cols < 4) continue;   // two dequantising groups
+          if (p.stages > cols) p.stages = cols;
+        }
+        double stage = kW4 ? (ctas == 1 ? 400 + 1.2 * bn : 380 + 0.86 * bn) : stage_bytes / 60.0;
+        if (kW4 && 2400.0 / p.stages > stage) stage = 2400.0 / p.stages;
+        if (!kW4 && stage < (ctas == 1 ? 200 : 295)) stage = ctas == 1 ? 200 : 295;
+        if (2.0 * bn > stage) stage = 2.0 * bn;
+        const double waves = (double)((tiles + room - 1) / room);
+        double cost = waves * (kUnit * p.units_per_split * stage) + 2000 + 8.0 * bn;
+        if (s > 1) cost += 4500 + 8.0 * bn;
+        if (best.bn == 0 || cost < best_cost) {
+          best = p;
+          best_cost = cost;
+        }
       }
     }
-  }
   if (cost_out) *cost_out = best_cost;
   return best;
 }
 
-template <bool kW4, bool kHalf, bool kGated>
+template <int kCtas, bool kW4, bool kHalf, bool kGated>
 int launch(const CUtensorMap& mx, const CUtensorMap& mw, const Args& a, cudaStream_t st) {
   static bool set[64] = {};  // per device: the attribute belongs to its context
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
+  const auto kernel = swap_gemm<kCtas, kW4, kHalf, kGated>;
   if (dev >= 64 || !set[dev]) {
-    e = cudaFuncSetAttribute(swap_gemm<kW4, kHalf, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<kW4>);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<kW4>);
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) set[dev] = true;
   }
   const int tiles = a.p.tiles_m * a.p.tiles_n;
-  const int clusters = a.p.splits > 1 || tiles < kPairs ? tiles : kPairs;
-  return launch_chained(swap_gemm<kW4, kHalf, kGated>, dim3(2 * a.p.splits * clusters), dim3(kThreads<kW4>), kSmem<kW4>, st,
-                        2 * a.p.splits, mx, mw, a);
+  const int teams = a.p.splits > 1 || tiles < kSms / kCtas ? tiles : kSms / kCtas;
+  return launch_chained(kernel, dim3(kCtas * a.p.splits * teams), dim3(kThreads<kW4>), kSmem<kW4>, st,
+                        kCtas * a.p.splits, mx, mw, a);
+}
+
+template <int kCtas, bool kW4>
+int launch_typed(const CUtensorMap& mx, const CUtensorMap& mw, const Args& a, int dtype, bool gated, cudaStream_t st) {
+  if (dtype == kFp16)
+    return gated ? launch<kCtas, kW4, true, true>(mx, mw, a, st) : launch<kCtas, kW4, true, false>(mx, mw, a, st);
+  return gated ? launch<kCtas, kW4, false, true>(mx, mw, a, st) : launch<kCtas, kW4, false, false>(mx, mw, a, st);
 }
 
 template <bool kW4>
@@ -614,17 +636,17 @@ int launch_any(const LinearArgs& l, const GemmPlan& p, const CUtensorMap& mw, in
   a.p = p;
   if ((long long)p.tiles_m * p.tiles_n > (1 << 28)) return MUSE_ERR_UNSUPPORTED_SHAPE;
   const uint32_t type = dtype == kBf16 ? 1u : 0u;  // operand format: 0 f16, 1 bf16
-  a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
-  a.b_bytes = (uint32_t)p.bn / 2 * 128;
+  a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.bn >> 3) << 17) |
+            ((uint32_t)(kTileM * p.ctas >> 4) << 24);
+  a.b_bytes = (uint32_t)p.bn / p.ctas * 128;
   auto vec = [](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
   a.out_vec = vec(l.out, l.ldo);
   a.add_vec = vec(l.add, l.ld_add);
   a.error_flag = error_flag;
   CUtensorMap mx;
-  const int rc = make_operand_map(&mx, DenseOperand{l.x, l.ldx, true}, l.tokens, l.cols, dtype, p.bn / 2);
+  const int rc = make_operand_map(&mx, DenseOperand{l.x, l.ldx, true}, l.tokens, l.cols, dtype, p.bn / p.ctas);
   if (rc) return rc;
-  if (dtype == kFp16) return gated ? launch<kW4, true, true>(mx, mw, a, st) : launch<kW4, true, false>(mx, mw, a, st);
-  return gated ? launch<kW4, false, true>(mx, mw, a, st) : launch<kW4, false, false>(mx, mw, a, st);
+  return p.ctas == 2 ? launch_typed<2, kW4>(mx, mw, a, dtype, gated, st) : launch_typed<1, kW4>(mx, mw, a, dtype, gated, st);
 }
 
 int padded_rows_of(const DenseGemm& g) { return (g.n + kTileM - 1) / kTileM * kTileM; }
