@@ -135,12 +135,24 @@ __device__ __forceinline__ void dgate4(const Args& p, int row, int col, float4 d
 // and b.
 template <int kMode> struct SideInput {
   uint2 add[8];
+  // every second 128-byte line of a row (the quarter's other warp takes the others)
+  static __device__ __forceinline__ void prefetch(const Args& p, int row, int col, int end) {
+    if (p.add)
+      for (; col < end; col += 128) prefetch_l2(static_cast<const uint16_t*>(p.add) + (size_t)row * p.ld_add + col);
+  }
   __device__ __forceinline__ void load(const Args& p, int i, int row, int col, bool more) {
     if (p.add && more && row < p.m && col < p.n) add[i] = load4(p.add, p.ld_add, row, col);
   }
 };
 template <> struct SideInput<kDGate> {
   float4 a[8], b[8];
+  static __device__ __forceinline__ void prefetch(const Args& p, int row, int col, int end) {
+    for (; col < end; col += 128)
+      for (int i = 0; i < 64 && col + i < end; i += 32) {
+        prefetch_l2(p.ab + (size_t)row * 2 * p.inter + col + i);
+        prefetch_l2(p.ab + (size_t)row * 2 * p.inter + p.inter + col + i);
+      }
+  }
   __device__ __forceinline__ void load(const Args& p, int i, int row, int col, bool more) {
     if (more && row < p.m && col < p.n) {
       const float* at = p.ab + (size_t)row * 2 * p.inter + col;
@@ -150,6 +162,7 @@ template <> struct SideInput<kDGate> {
   }
 };
 template <> struct SideInput<kGate> {
+  static __device__ __forceinline__ void prefetch(const Args&, int, int, int) {}
   __device__ __forceinline__ void load(const Args&, int, int, int, bool) {}
 };
 
@@ -294,9 +307,12 @@ dense_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
     for (int w = pair; w < total; w += pairs, ++it) {
       const Tile t = tile_of(a, w);
       const int buf = it & 1;
-      // what the first patch is combined with, fetched while its sums are still being taken
+      // what the tile is combined with starts for L2, and for the first patch for registers, while the
+      // sums are still being taken
       SideInput<kMode> side;
       if (!t.partial) {
+        const int row = t.m0 + rank * kBm + quarter * 32 + lane;
+        if (row < a.m) SideInput<kMode>::prefetch(a, row, t.n0 * a.bn + half * 64, min(a.n, (t.n0 + 1) * a.bn));
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           side.load(a, i, t.m0 + rank * kBm + quarter * 32 + 4 * i + rr, t.n0 * a.bn + 32 * half + cc, true);

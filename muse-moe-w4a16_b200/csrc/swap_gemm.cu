@@ -255,7 +255,11 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   auto first_addend = [&](const Tile& t) {
     const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
     const int outs = min(kOut, a.l.n_out - o0), n_tok = min(a.p.bn, a.l.tokens - t.tok0);
-    if (a.l.add && outs > 0 && 32 * split < n_tok)
+    if (!a.l.add || outs <= 0) return;
+    // the warp's rows of this tile's addend start for L2 together, while the sums are still being taken
+    for (int tok = 32 * split + lane; tok < n_tok; tok += step)
+      prefetch_l2(a.l.add + (size_t)(t.tok0 + tok) * a.l.ld_add + o0);
+    if (32 * split < n_tok)
       Io::load(ahead, lane, a.l.add + o0, a.l.ld_add, t.tok0 + 32 * split, min(32, n_tok - 32 * split), outs, a.add_vec);
   };
   auto tile_epilogue = [&](const Tile& t, int buf) {
