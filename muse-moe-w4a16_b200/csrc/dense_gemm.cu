@@ -105,7 +105,7 @@ __device__ __forceinline__ void store4(int dtype, void* base, long long ld, int 
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + (size_t)row * ld + col) = p;
 }
 __device__ __forceinline__ uint2 load4(const void* base, long long ld, int row, int col) {
-  return __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + (size_t)row * ld + col));
+  return __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + (size_t)row * ld + col));
 }
 __device__ __forceinline__ float4 add4(int dtype, uint2 p, float4 v) {
   const float2 lo = unpack16(dtype, p.x), hi = unpack16(dtype, p.y);
@@ -156,8 +156,8 @@ template <> struct SideInput<kDGate> {
   __device__ __forceinline__ void load(const Args& p, int i, int row, int col, bool more) {
     if (more && row < p.m && col < p.n) {
       const float* at = p.ab + (size_t)row * 2 * p.inter + col;
-      a[i] = __ldg(reinterpret_cast<const float4*>(at));
-      b[i] = __ldg(reinterpret_cast<const float4*>(at + p.inter));
+      a[i] = __ldcg(reinterpret_cast<const float4*>(at));
+      b[i] = __ldcg(reinterpret_cast<const float4*>(at + p.inter));
     }
   }
 };
@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(256) dense_reduce(const Args a) {
       store4(a.dtype, a.out, a.ldo, row, col, x);
     } else if (kMode == kDGate) {
       const float* at = a.ab + (size_t)row * 2 * a.inter + col;
-      dgate4(a, row, col, x, __ldg(reinterpret_cast<const float4*>(at)),
-             __ldg(reinterpret_cast<const float4*>(at + a.inter)));
+      dgate4(a, row, col, x, __ldcg(reinterpret_cast<const float4*>(at)),
+             __ldcg(reinterpret_cast<const float4*>(at + a.inter)));
     } else {
       if (a.add) x = add4(a.dtype, load4(a.add, a.ld_add, row, col), x);
       store4(a.dtype, a.out, a.ldo, row, col, x);

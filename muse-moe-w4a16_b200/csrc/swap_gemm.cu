@@ -145,11 +145,11 @@ struct PatchIo {
       if (tok >= toks) continue;
       const uint16_t* g = base + (size_t)(tok0 + tok) * ld + 8 * p;
       if (vec && 8 * p + 8 <= outs) {
-        v[i] = __ldg(reinterpret_cast<const uint4*>(g));
+        v[i] = __ldcg(reinterpret_cast<const uint4*>(g));
       } else {
         uint32_t e[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = 8 * p + j < outs ? __ldg(g + j) : 0;
+        for (int j = 0; j < 8; ++j) e[j] = 8 * p + j < outs ? __ldcg(g + j) : 0;
         v[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
       }
     }

@@ -83,8 +83,9 @@ template <bool kHalf> constexpr float kUnscale = kHalf ? 1.f : 256.f;
 
 
 __device__ __forceinline__ uint16_t round16(int dtype, float v) { return (uint16_t)(pack16(dtype, v, v) & 0xFFFF); }
+// (from L2: an addend may be the output that the kernel before wrote in place)
 __device__ __forceinline__ float load16(int dtype, const uint16_t* p) {
-  return unpack16(dtype, (uint32_t)__ldg(p)).x;
+  return unpack16(dtype, (uint32_t)__ldcg(p)).x;
 }
 
 }  // namespace muse

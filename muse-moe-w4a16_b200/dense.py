@@ -19,6 +19,7 @@ from . import _lib
 from .layer import _require_cuda
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_MAX_ROWS = 1 << 28   # rows of x in one call
 
 
 class LinearWeights(TypedDict):
@@ -132,6 +133,8 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
         raise _bad("linear_w4 has no gradient: call it under torch.no_grad()")
     x2, ldx = _rows(x, K)
     T = x2.shape[0]
+    if T > _MAX_ROWS:
+        raise _lib.MuseError(_lib.MUSE_ERR_UNSUPPORTED_SHAPE, f"{T} rows in one call, at most {_MAX_ROWS}")
     if len(shape) == 2:
         shape = (T, n_out)
     else:
@@ -242,6 +245,8 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, add: torch.T
         raise _bad(f"inconsistent shapes: x {tuple(x.shape)}, w13 {tuple(w13.shape)}, w2 {tuple(w2.shape)}")
     if H == 0 or I == 0 or H % 8 or I % 8:
         raise _lib.MuseError(_lib.MUSE_ERR_UNSUPPORTED_SHAPE, f"H = {H} and I = {I} must be multiples of 8")
+    if x.numel() // H > _MAX_ROWS:
+        raise _lib.MuseError(_lib.MUSE_ERR_UNSUPPORTED_SHAPE, f"{x.numel() // H} rows in one call, at most {_MAX_ROWS}")
     if add is not None:
         _same(add, "add", dev, x.dtype)
         if add.shape != x.shape:

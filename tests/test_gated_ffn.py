@@ -137,6 +137,21 @@ def test_only_wanted_gradients(pkg, which):
 
 
 @gpu
+def test_gradient_of_the_addend_alone(pkg):
+    x, w13, w2, dy, add = make(20, 64, 72, torch.bfloat16)
+    leaf = add.clone().requires_grad_()
+    y = pkg.gated_ffn(x, w13, w2, add=leaf)
+    y.backward(dy)
+    assert torch.equal(leaf.grad, dy) and torch.equal(y.detach(), pkg.gated_ffn(x, w13, w2, add=add))
+    # one tensor as input and addend: both gradients reach it
+    both = x.clone().requires_grad_()
+    pkg.gated_ffn(both, w13, w2, add=both).backward(dy)
+    only = x.clone().requires_grad_()
+    pkg.gated_ffn(only, w13, w2).backward(dy)
+    assert torch.equal(both.grad, only.grad + dy)
+
+
+@gpu
 def test_empty(pkg):
     _, w13, w2, _, _ = make(1, 64, 72, torch.bfloat16)
     x = torch.empty((0, 64), dtype=torch.bfloat16, device=DEV, requires_grad=True)

@@ -51,6 +51,7 @@ def test_entry_refuses_before_any_launch(pkg):
                 dict(x=264), dict(ldx=68), dict(ldx=56), dict(ldo=31), dict(add=256, ld_add=31)):
         assert call(**bad) == -1, bad
     assert call(cols=40) == -2
+    assert call(tokens=(1 << 28) + 1) == -2
 
 
 # ------------------------------------------------------------------ parity
@@ -130,6 +131,8 @@ def test_strides_shapes_and_out(pkg, T):
                 lambda: pkg.linear_w4(x, state, out=x.view(-1)[:T * 300].view(T, 300))):
         with pytest.raises(pkg.MuseError):
             bad()
+    assert torch.equal(pkg.linear_w4(x[0], state, add=add[0]), y[0]) or T > 8   # (fewer rows, another kernel)
+    assert pkg.linear_w4(x[0], state).shape == (300,)
     one = x[:1].expand(T, 512)
     assert torch.equal(pkg.linear_w4(one, state), pkg.linear_w4(one.contiguous(), state))
 
