@@ -103,3 +103,44 @@ def test_trained_in_sixteen_bits_served_in_four(pkg):
         h = pkg.linear_w4(x, pkg.prepare_linear(q13, gated=True))
         ref.check(h, *ref.linear64(x, q13, True), "4 bits, inner")
         ref.check(pkg.linear_w4(h, pkg.prepare_linear(q2)), *ref.linear64(h, q2, False), "4 bits")
+
+
+@pytest.mark.parametrize("T", [2, 14, 70, 300])
+def test_long_chains_on_two_streams(pkg, T):
+    """Hundreds of dependent calls with nothing between them, their temporaries' memory handed from call
+    to call, in place on an addend, on two streams at once: every repeat gives the first one's bits."""
+    H, I = 384, 256
+    g = torch.Generator().manual_seed(T)
+    q1 = quantised(torch.randn((2 * I, H), generator=g) * H ** -0.5)
+    q2 = quantised(torch.randn((H, I), generator=g) * I ** -0.5)
+    s13 = pkg.prepare_linear({k: v.to(DEV) for k, v in q1.items()}, gated=True)
+    s2 = pkg.prepare_linear({k: v.to(DEV) for k, v in q2.items()})
+    f13 = (torch.randn((2 * I, H), generator=g) * H ** -0.5).to(torch.bfloat16).to(DEV)
+    f2 = (torch.randn((H, I), generator=g) * I ** -0.5).to(torch.bfloat16).to(DEV)
+    x = torch.randn((T, H), generator=g).to(torch.bfloat16).to(DEV)
+
+    @torch.no_grad()
+    def chain():
+        y = x.clone()
+        for _ in range(4):
+            pkg.linear_w4(pkg.linear_w4(y, s13), s2, add=y, out=y)
+            y = pkg.gated_ffn(y, f13, f2, add=y)
+            y = y / y.float().square().mean().sqrt().to(y.dtype)
+        return y
+
+    def gradients():
+        leaves = [t.detach().requires_grad_() for t in (x, f13, f2)]
+        return torch.autograd.grad(pkg.gated_ffn(*leaves), leaves, x)
+
+    want, want_g = chain(), gradients()
+    torch.cuda.synchronize()
+    outs = []
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append((chain(), gradients()))
+    torch.cuda.synchronize()
+    for y, grads in outs:
+        assert torch.equal(y, want)
+        for a, b in zip(grads, want_g):
+            assert torch.equal(a, b)
