@@ -115,6 +115,6 @@ extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int t
   const cudaStream_t st = (cudaStream_t)stream;
   int* flag = nullptr;
   if ((rc = device_status_ptr(&flag))) return rc;
-  if (tokens <= kFewTokens) return launch_few_w4(a, dtype, gated, flag, st);
+  if (streams_w4(tokens, rows, cols)) return launch_few_w4(a, dtype, gated, flag, st);
   return launch_linear_gemm(a, dtype, gated, flag, st);
 }
