@@ -201,41 +201,34 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   const int team = blockIdx.x / (kCtas * splits), teams = gridDim.x / (kCtas * splits);
   const int total = a.p.tiles_m * a.p.tiles_n;
 
-  // The first codes are fetched before anything else: they depend on no other CTA, and prepare alone
-  // writes them, so not on the kernel before either.
-  auto load_codes = [&](const Tile& t, int c, int slot) {
-    // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
-    const int m = min(t.m_tile, a.l.padded_rows / kTileM - 1);
-    ptx::mbar_arrive_expect_tx(&ctl.code_full[slot], kCodeBytes);
-    ptx::bulk_g2s(codes + slot * kCodeBytes, a.l.wq + ((size_t)m * a.p.units + c) * kLinearTileBytes, kCodeBytes,
-                  &ctl.code_full[slot]);
-  };
-  int early = 0;
-  if (kW4 && threadIdx.x == 0) {
-    for (int s = 0; s < kCodes; ++s) {
-      ptx::mbar_init(&ctl.code_full[s], 1);
-      ptx::mbar_init(&ctl.code_empty[s], 4);
+  // Barriers, one lane each.
+  if (warp == 0) {
+    if (kW4 && lane < kCodes) {
+      ptx::mbar_init(&ctl.code_full[lane], 1);
+      ptx::mbar_init(&ctl.code_empty[lane], 4);
     }
     ptx::fence_barrier_init();
-    const Tile t = tile_of<kCtas>(a.p, team, rank, split);
-    for (; early < kCodes && t.c0 + early < t.c1; ++early) load_codes(t, t.c0 + early, early);
-  }
-  if (threadIdx.x == 64) {
-    for (int s = 0; s < n_stages; ++s) {
-      ptx::mbar_init(&ctl.full[s], kW4 ? 1 + kCtas * 4 : 1);  // bytes announced by the leader; NVFP4's A by four warps of each CTA
-      ptx::mbar_init(&ctl.empty[s], 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      ptx::mbar_init(&ctl.acc_full[b], 1);
-      ptx::mbar_init(&ctl.acc_empty[b], kCtas * 4);
+  } else if (warp == 1) {
+    G::alloc(&ctl.tmem, kTmemCols);
+  } else if (warp == 2) {
+    if (lane < n_stages) {
+      ptx::mbar_init(&ctl.full[lane], kW4 ? 1 + kCtas * 4 : 1);  // bytes announced by the leader; NVFP4's A by four warps of each CTA
+      ptx::mbar_init(&ctl.empty[lane], 1);
+    } else if (lane < n_stages + 2) {
+      ptx::mbar_init(&ctl.acc_full[lane - n_stages], 1);
+      ptx::mbar_init(&ctl.acc_empty[lane - n_stages], kCtas * 4);
     }
     ptx::fence_barrier_init();
-    ptx::prefetch_tensormap(&map_x);
+    if (lane == 0) ptx::prefetch_tensormap(&map_x);
   }
-  if (warp == 1) G::alloc(&ctl.tmem, kTmemCols);
   ptx::tc_fence_before();
   __syncthreads();
-  if (kCtas * splits > 1) cluster_sync();
+  // A pair's CTAs use each other's barriers from the start, which codes do not need: their warp goes on.
+  // Groups meet when they exchange sums.
+  if (kCtas > 1) {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    if (warp > 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
   ptx::tc_fence_after();
   const uint32_t tmem = ctl.tmem;
   // tensor memory: one accumulator (two where a pair has several tiles), then NVFP4's A stages
@@ -353,22 +346,24 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
 
   if (warp == 0) {
     if (kW4 && lane == 0) {
+      // codes: written by prepare only, so they are fetched without waiting for the kernel before
       Pos q;
       for (int w = team; w < total && ok; w += teams) {
         const Tile t = tile_of<kCtas>(a.p, w, rank, split);
+        // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
+        const uint8_t* src = a.l.wq + (size_t)min(t.m_tile, a.l.padded_rows / kTileM - 1) * a.p.units * kLinearTileBytes;
         for (int c = t.c0; c < t.c1; ++c, q.next(kCodes)) {
-          if (early > 0) {   // already on its way
-            --early;
-            continue;
-          }
           if (!ptx::mbar_wait_sleep(&ctl.code_empty[q.slot], q.phase ^ 1)) {
             ok = false;
             break;
           }
-          load_codes(t, c, q.slot);
+          ptx::mbar_arrive_expect_tx(&ctl.code_full[q.slot], kCodeBytes);
+          ptx::bulk_g2s(codes + q.slot * kCodeBytes, src + (size_t)c * kLinearTileBytes, kCodeBytes, &ctl.code_full[q.slot]);
         }
       }
     }
+    __syncwarp();
+    if (kCtas > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   } else if (warp == 1) {
     if (rank == 0 && ptx::elect_one()) {
       chain_wait();   // B comes after it: the bounded waits do not count the kernel before
