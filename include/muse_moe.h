@@ -73,7 +73,8 @@ int muse_moe_workspace_offsets(int tokens, int top_k, int local_count, int hidde
  * failure (then a call returned garbage): 1-4 a wait of the expert GEMM's producer / MMA /
  * epilogue / dequantiser role expired, 5 the single launch's combine waited in vain for its
  * rows, 6 an expert-parallel exchange waited in vain for a peer, 7 an exchange found the
- * device's generation parity different from the caller's, 8 a wait of a dense product expired. Synchronous: copies from the device
+ * device's generation parity different from the caller's, 8 a wait of a dense product expired.
+ * Synchronous: copies from the device
  * on the current device; reset != 0 clears it. Not for use inside a captured graph.
  */
 int muse_moe_device_status(int* status, int reset);

@@ -4,14 +4,16 @@
 // A CTA takes 128 weight rows (gated 16-bit weights: 64 gate rows and the 64 matching up rows) and a
 // cluster of CTAs splits K. One thread copies the weights into a ring of shared memory, 128 codes
 // or 64 16-bit columns to a stage (one bulk copy of a tile, or a TMA box), and the same columns of
-// x (TMA; rows past the last token read as zeros). Eight warps multiply 16 rows each (from nine
-// tokens on 32 rows and half of the k) by mma.sync m16n8k16: tokens are the 8-wide side, so one token wastes no weight traffic, and at 32 tokens the
-// matrix pipe still keeps up with HBM. Lanes read both operands as 16-byte pieces along k -- the order of k inside a
-// stage is the lanes' -- so nothing is shuffled. A CTA pushes its sums to the ranks that own the
-// outputs (16-byte stores to distributed shared memory, one cluster barrier), which add them in
-// rank order. Sixteen warps with half of a stage each measured slower (13.0 against 8.7 us at 1 x 7168 x
-// 4096 gated): for NVFP4 the instructions per code are what keeps the stream from HBM's rate.
-// Bound by the weights' bytes; the smallest sizes by launch, first-byte and cluster latency.
+// x (TMA; rows past the last token read as zeros). Eight warps multiply 16 rows each (9 to 16 tokens:
+// 32 rows and half of the k) by mma.sync m16n8k16: tokens are the 8-wide side, so one token wastes no
+// weight traffic. Lanes read both operands as 16-byte pieces along k -- the order of k inside a stage
+// is the lanes' -- so nothing is shuffled. A CTA pushes its sums to the ranks that own the outputs
+// (16-byte stores to distributed shared memory, one cluster barrier), which add them in rank order.
+// Sixteen warps with half of a stage each measured slower (13.0 against 8.7 us at 1 x 7168 x 4096
+// gated): for NVFP4 the instructions per code are what keeps the stream from HBM's rate.
+// Bound by the weights' bytes (the block of 1 x 7168 x 2048 in 16 bits: 20.0 us, 4.4 TB/s over both
+// products; NVFP4 1 x 7168 x 4096 gated: 8.8 us, 1.9 TB/s); the smallest sizes by launch, first-byte
+// and cluster latency (1 x 1024 x 1024: 3.2 us).
 #undef MUSE_TRACE  // these kernels record no stamps
 #include "few_tokens.cuh"
 

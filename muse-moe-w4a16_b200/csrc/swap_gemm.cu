@@ -13,16 +13,18 @@
 //   weight row) and store them to tensor memory, from where the MMAs read A. Through shared memory,
 //   which carries B, the codes and its own 16 KiB twice, a stage took ~450 clocks at 64 tokens and
 //   ~630 at 256.
-// Accumulators are double buffered in tensor memory; the epilogue reads them as matrix fragments
+// Where a group has several tiles its accumulators are double buffered in tensor memory, so that the
+// epilogue overlaps the next tile's MMAs; it reads them as matrix fragments
 // and turns them over (rows are weight rows, y's rows are tokens) with transposed matrix stores
 // into shared memory, so that global stores run along y's rows. Gated tiles hold gate and up rows
 // of an output in one thread's fragments.
 // With fewer tiles than groups K is split over the groups (CTAs or pairs) of a cluster of up to eight
 // CTAs. Each group owns every splits-th 32-token chunk of the tile's outputs and receives the others'
-// accumulators of it, as fragments, through distributed shared memory (the rings are done by then): the owner adds
-// them to its own in split order and finishes the chunk. One launch, no scratch memory.
-// Bound by weight bytes (NVFP4: and the dequantisation) for tens of tokens, by the tensor pipe for
-// hundreds.
+// accumulators of it, as fragments, through distributed shared memory (the rings are done by then): the
+// owner adds them to its own, in split order, and finishes the chunk. One launch, no scratch memory.
+// Tens of tokens are bound by set-up, exchange and the dequantisation more than by weight bytes (64 x
+// 4096 x 8192 gated: 14.4 us, 1.4 TB/s), hundreds by the tensor pipe (1000 x 4096 x 4096: 32 us; 2000 x
+// 7168 x 4096 gated: 100 us, 1.17 PFLOP/s, in a loop under the power limit).
 #undef MUSE_TRACE  // these kernels record no stamps
 #include "kernels.cuh"
 #include "pair.cuh"
@@ -35,8 +37,8 @@ constexpr int kMaxStages = 12;
 constexpr int kABytes = kTileM * 128;
 constexpr int kCodes = 8;                    // code ring: 128-code chunks of 9 KiB
 constexpr int kCodeBytes = kLinearTileBytes;
-// 64-k stages in shared memory: B (128 bytes a token; half the tokens in a pair) and, 16-bit weights, A (16 KiB). NVFP4's A
-// takes 32 columns of tensor memory.
+// 64-k stages in shared memory: B (128 bytes a token; half the tokens in a pair) and, 16-bit weights,
+// A (16 KiB). NVFP4's A takes 32 columns of tensor memory.
 template <bool kW4> constexpr int kRingBytes = kW4 ? 8 * kABytes : 13 * kABytes;
 template <bool kW4> constexpr int kStageA = kW4 ? 0 : kABytes;
 constexpr int kTmemCols = 512;
@@ -231,18 +233,18 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   }
   ptx::tc_fence_after();
   const uint32_t tmem = ctl.tmem;
-  // tensor memory: one accumulator (two where a pair has several tiles), then NVFP4's A stages
+  // tensor memory: one accumulator (two where a group has several tiles), then NVFP4's A stages
   const uint32_t a_cols = tmem + a.p.accs * a.p.bn;
   chain_release();
 
   bool ok = true;
-  // ---- epilogue of a tile: this pair's chunks of 32 tokens (all of them unless K is split)
+  // ---- epilogue of a tile: this group's chunks of 32 tokens (all of them unless K is split)
   constexpr int dtype = kHalf ? kFp16 : kBf16;
   constexpr int kOut = kGated ? 16 : 32;                  // outputs of an epilogue warp
   using Io = PatchIo<kOut>;
   const int quarter = warp & 3, epi = warp - kEpiWarp0<kW4>, step = 32 * splits;
   const int chunks = (a.p.bn / 32 + splits - 1) / splits; // most chunks of one owner
-  // another pair's fragments of this pair's chunk `i` (of pair `from`, without the owner itself)
+  // fragments of this group's chunk `i` from another group (`from` counts the others)
   auto received = [&](uint8_t* base, int from, int i) { return base + (((from * chunks + i) * 4 + epi) << 12) + lane * 16; };
   uint4 ahead[Io::kPieces];                               // the next patch's addend
   auto first_addend = [&](const Tile& t) {
@@ -509,7 +511,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   __syncwarp();
   if (splits > 1) {
     const Tile t = tile_of<kCtas>(a.p, team, rank, split);
-    cluster_sync();   // every pair's MMAs are done, and with them the reads of the rings
+    cluster_sync();   // every group's MMAs are done, and with them the reads of the rings
     if (warp >= kEpiWarp0<kW4>) {
       const uint32_t acc = tmem + ((uint32_t)quarter << 21);
       const int n_tok = min(a.p.bn, a.l.tokens - t.tok0);
