@@ -350,11 +350,16 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
     if (kW4 && lane == 0) {
       // codes: written by prepare only, so they are fetched without waiting for the kernel before
       Pos q;
+      bool ahead_of_it = true;
       for (int w = team; w < total && ok; w += teams) {
         const Tile t = tile_of<kCtas>(a.p, w, rank, split);
         // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
         const uint8_t* src = a.l.wq + (size_t)min(t.m_tile, a.l.padded_rows / kTileM - 1) * a.p.units * kLinearTileBytes;
         for (int c = t.c0; c < t.c1; ++c, q.next(kCodes)) {
+          if (ahead_of_it && q.phase) {   // the ring is full: the bounded waits begin
+            chain_wait();
+            ahead_of_it = false;
+          }
           if (!ptx::mbar_wait_sleep(&ctl.code_empty[q.slot], q.phase ^ 1)) {
             ok = false;
             break;
