@@ -4,7 +4,7 @@ weights, with gradients).
 Both are what a layer with routed experts needs next to them: its dense projections and its
 shared expert, whose output is added to the routed one (`add`). Same rules as kernel_fn: CUDA
 tensors only, the current stream, memory from torch's caching allocator, no host
-synchronisation; so calls can be captured in a CUDA graph after one eager call.
+synchronisation; so calls can be captured in a CUDA graph after one eager call of the same sizes.
 """
 
 from __future__ import annotations
@@ -14,6 +14,7 @@ import functools
 from typing import TypedDict
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .layer import _require_cuda
@@ -85,7 +86,11 @@ def _rows(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
 
 def prepare_linear(weight: LinearWeights, gated: bool = False) -> dict:
     """Repack an NVFP4 matrix [N, K] for linear_w4 (once, untimed): any N, K a multiple of 16.
-    gated: rows [0, N/2) are gate rows and the rest the matching up rows (a w13)."""
+    gated: rows [0, N/2) are gate rows and the rest the matching up rows (a w13).
+
+    The state's tensors may be copied and rewritten in place like any others, but not by a kernel
+    that lets its successor start early (programmatic dependent launch; torch's own do not):
+    linear_w4 begins to read the weight ahead of the end of such a kernel."""
     w, sf, gs = weight["w"], weight["w_sf"], weight["w_gs"]
     _require_cuda(w, "w")
     if w.dtype != torch.uint8 or w.dim() != 2 or 0 in w.shape:
@@ -127,8 +132,9 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
     shape = x.shape
     if not shape or shape[-1] != K:
         raise _bad(f"x {tuple(shape)} does not end in the weight's {K} columns")
-    if w.device != dev:
-        raise _bad(f"the weight is on {w.device}, x on {dev}")
+    gs = state["w_gs"]
+    if w.device != dev or gs.device != dev:
+        raise _bad(f"the weight is on {w.device} and its scale on {gs.device}, x on {dev}")
     if torch.is_grad_enabled() and (x.requires_grad or (add is not None and add.requires_grad)):
         raise _bad("linear_w4 has no gradient: call it under torch.no_grad()")
     x2, ldx = _rows(x, K)
@@ -155,8 +161,12 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
     elif _overlap(out, x) or (add is not None and _overlap(out, add)
                               and (add.data_ptr() != out.data_ptr() or not add.is_contiguous())):
         raise _bad("out may be add itself, but overlaps no input otherwise")
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise _bad("out requires a gradient, which linear_w4 does not have")
+    else:
+        increment_version(out)   # autograd sees the write: a backward pass that kept out's old values refuses
     _call(dev.index, "muse_moe_linear_w4", x2.data_ptr(), ldx, dtype, T, state["rows"], K, 1 if state["gated"] else 0,
-          w.data_ptr(), state["w_gs"].data_ptr(), add_ptr, ld_add, out.data_ptr(), n_out)
+          w.data_ptr(), gs.data_ptr(), add_ptr, ld_add, out.data_ptr(), n_out)
     return out
 
 

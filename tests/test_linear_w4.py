@@ -206,3 +206,50 @@ def test_graph_stream_and_repeat(pkg, T):
             g.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 12, 70, 400])
+def test_weights_rewritten_in_place(pkg, T):
+    """A kernel rewrites the prepared weight between calls, with nothing between the launches: each call
+    sees the weight as it is at its place in the stream."""
+    x, state, _, y = run(pkg, T, 384, 1024, True, torch.bfloat16, False, seed=5)
+    other = pkg.prepare_linear(ref.random_w4(384, 1024, 6, DEV), gated=True)
+    z = pkg.linear_w4(x, dict(other, w_gs=state["w_gs"]))
+    flip = state["w"] ^ other["w"]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(40):
+        state["w"].bitwise_xor_(flip)
+        outs += [pkg.linear_w4(x, state), pkg.linear_w4(x, state)]
+    torch.cuda.synchronize()
+    assert not torch.equal(y, z)
+    for i, got in enumerate(outs):
+        assert torch.equal(got, y if i // 2 % 2 else z), i
+
+
+@gpu
+def test_out_and_autograd(pkg):
+    """A leaf that wants a gradient is refused as out; writing over what a backward pass keeps is noticed."""
+    state = pkg.prepare_linear(ref.random_w4(64, 64, 1, DEV))
+    x = torch.ones((2, 64), dtype=torch.bfloat16, device=DEV)
+    out = torch.ones_like(x)
+    leaf = torch.ones_like(x).requires_grad_()
+    with pytest.raises(pkg.MuseError) as e:
+        pkg.linear_w4(x, state, out=leaf)
+    assert e.value.code == -1
+    y = leaf * out
+    pkg.linear_w4(x, state, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.no_grad():
+        pkg.linear_w4(x, state, out=leaf)
+    assert torch.equal(out, leaf)
+
+
+@gpu
+def test_scale_on_another_device_is_refused(pkg):
+    state = pkg.prepare_linear(ref.random_w4(64, 64, 1, DEV))
+    with pytest.raises(pkg.MuseError) as e:
+        pkg.linear_w4(torch.zeros((2, 64), dtype=torch.bfloat16, device=DEV), dict(state, w_gs=state["w_gs"].cpu()))
+    assert e.value.code == -1
