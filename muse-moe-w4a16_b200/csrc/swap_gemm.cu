@@ -457,9 +457,6 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
 #pragma unroll
       for (int k = 0; k < 4; ++k) code[k] = *reinterpret_cast<const uint4*>(src + r * kRowCodeBytes + 16 * code_slot(r, k));
       sc = *reinterpret_cast<const uint2*>(src + kTileCodeBytes + r * kRowScaleBytes);
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&ctl.code_empty[q.slot]);
-      q.skip(groups, kCodes);
     };
     if (group < n) fetch();
     for (int i = group; i < n && ok; i += groups) {
@@ -482,6 +479,12 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
         slots[h] = at.slot;
         at.next(n_stages);
       }
+      // The slot is given back only here, where the stores have taken what was made of the loaded values.
+      // An arrival does not wait for loads before it: with the epilogue's accesses to a large output
+      // in the queue ahead of them (2^20 tokens) the next copy overtook them.
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&ctl.code_empty[q.slot]);
+      q.skip(groups, kCodes);
       if (i + groups < n) fetch();  // while the stores are on their way
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
