@@ -253,3 +253,22 @@ def test_scale_on_another_device_is_refused(pkg):
     with pytest.raises(pkg.MuseError) as e:
         pkg.linear_w4(torch.zeros((2, 64), dtype=torch.bfloat16, device=DEV), dict(state, w_gs=state["w_gs"].cpu()))
     assert e.value.code == -1
+
+
+@gpu
+def test_a_million_tokens_repeat(pkg):
+    """Offsets past 32 bits, and the same bits from repeats and in place on the addend: copies and waits
+    take longest at this size."""
+    T, N, K = (1 << 20) + 77, 2064, 2048
+    weight = ref.random_w4(N, K, 1, DEV)
+    state = pkg.prepare_linear(weight)
+    x = torch.randn((T, K), dtype=torch.bfloat16, device=DEV)
+    add = torch.randn((T, N), dtype=torch.bfloat16, device=DEV)
+    y = pkg.linear_w4(x, state, add=add)
+    for _ in range(3):
+        assert torch.equal(pkg.linear_w4(x, state, add=add), y)
+    for first in (0, T // 2, T - 40):
+        rows = slice(first, first + 40)
+        ref.check(y[rows], *ref.linear64(x[rows], weight, False, add[rows]), f"rows from {first}")
+    pkg.linear_w4(x, state, add=add, out=add)
+    assert torch.equal(add, y)
