@@ -814,8 +814,8 @@ expert_gemm_tc(const __grid_constant__ CUtensorMap tmap_b, const __grid_constant
     // memory reads of group g + 1 -- its 16 code bytes and its two scale-table entries -- are
     // issued before group g is converted, so their latency hides behind the arithmetic; the
     // reads of the next chunk's first group are issued during the last group whenever that
-    // weight tile has already landed. A weight slot is handed back as soon as its last bytes
-    // are in registers, and the A buffer is waited for only once the first group is converted.
+    // weight tile has already landed. A weight slot is handed back once the stores of its last
+    // group have taken the values, and the A buffer is waited for only once the first group is converted.
     const int p = (warp - kDeqWarp0) / DW;
     PipeCtl& pc = ctl.pipe[p];
     const int q = warp & 3;                  // TMEM lane quarter
@@ -890,9 +890,7 @@ expert_gemm_tc(const __grid_constant__ CUtensorMap tmap_b, const __grid_constant
           cn = load_codes(cur, g + 1);
           lut(sfw, g + 1, n0, n1);
         } else {
-          // every byte of this chunk is read: hand the slot back, then look ahead
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(&pc.w_empty[cur]);
+          // the chunk's last reads are issued: look ahead into the next slot
           st.next(Sw);
           more_next = advance();
           if (more_next && __all_sync(0xffffffffu, ptx::mbar_try_wait(&pc.w_full[st.slot], st.phase))) {
@@ -911,6 +909,13 @@ expert_gemm_tc(const __grid_constant__ CUtensorMap tmap_b, const __grid_constant
           break;
         }
         ptx::tmem_st16(lane_col0 + ab * kACols + hsel * 32 + g * 16, out);
+        // Only now has every lane's last code value arrived in its registers (the store took what was
+        // made of it), so the slot goes back. An arrival does not wait for loads that precede it: the
+        // next copy could overtake them where the memory pipeline is backed up.
+        if (g + 1 == kGroups) {
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&pc.w_empty[cur]);
+        }
         cg = cn;
         s0 = n0;
         s1 = n1;
