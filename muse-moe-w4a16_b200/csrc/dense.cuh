@@ -92,9 +92,8 @@ __device__ __forceinline__ float2 unpack16(int dtype, uint32_t v) {
 // ---- programmatic dependent launch: the kernels of one call are launched with the attribute
 // (launch_chained) and wait here before they touch global memory, so a kernel's set-up overlaps
 // the one before it. Every thread that reads or writes global memory waits, and does so before its
-// bounded waits. One exception: codes of prepared weights are copied ahead of the wait. A kernel that
-// does not release its dependents early (prepare_linear's and torch's do not) has ended by then, so
-// only a kernel that does, and writes prepared weights, would be read too soon; there is none here.
+// bounded waits: what the kernel before wrote is visible only after the wait, even where it releases
+// nothing early and its CTAs have left. Ahead of it weights are at most drawn into L2.
 
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -113,13 +113,13 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
       ptx::tma_load_2d(dst, &map_x, k * kK, 0, &ctl.full[slot]);
       if (kW4) ptx::tma_load_2d(dst + kNT * 1024, &map_x, k * kK + 64, 0, &ctl.full[slot]);
     };
-    // Ahead of the wait for the kernel before: prepared weights (written by prepare only) are
-    // copied, 16-bit weights, which that kernel might have written, only drawn into L2.
+    // Ahead of the wait for the kernel before, which might have written the weights, they are only drawn
+    // into L2: a copy into shared memory would keep what it read too early.
     const int head = min(n_stages, a.depth);
     if (leader) {
       for (int i = 0; i < head; ++i) {
         if (kW4) {
-          load_w(i);
+          prefetch_bulk(a.wq + ((size_t)m_tile * a.stages + first + i) * kWBytes, kWBytes);
         } else {
           prefetch_tile(&map_w, (first + i) * kK, m_tile * kOut);
           if (kGated) prefetch_tile(&map_w, (first + i) * kK, a.up_row + m_tile * 64);
@@ -127,7 +127,7 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
       }
       chain_wait();
       for (int i = 0; i < head; ++i) {
-        if (!kW4) load_w(i);
+        load_w(i);
         load_x(i);
       }
     }

@@ -50,6 +50,10 @@ __device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int c0, in
                "r"(c0), "r"(c1)
                : "memory");
 }
+// Contiguous bytes into L2 only (address and size multiples of 16).
+__device__ __forceinline__ void prefetch_bulk(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"

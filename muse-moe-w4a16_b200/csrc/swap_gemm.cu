@@ -225,7 +225,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   }
   ptx::tc_fence_before();
   __syncthreads();
-  // A pair's CTAs use each other's barriers from the start, which codes do not need: their warp goes on.
+  // A pair's CTAs use each other's barriers from the start, which the codes' warp does not: it goes on.
   // Groups meet when they exchange sums.
   if (kCtas > 1) {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -348,18 +348,22 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
 
   if (warp == 0) {
     if (kW4 && lane == 0) {
-      // codes: written by prepare only, so they are fetched without waiting for the kernel before
+      // The kernel before might have written the weight: ahead of it the first codes are only drawn into L2.
+      auto tile_codes = [&](int m_tile) {
+        // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
+        return a.l.wq + (size_t)min(m_tile, a.l.padded_rows / kTileM - 1) * a.p.units * kLinearTileBytes;
+      };
+      if (team < total) {
+        const Tile t = tile_of<kCtas>(a.p, team, rank, split);
+        for (int c = t.c0; c < min(t.c1, t.c0 + kCodes); ++c)
+          prefetch_bulk(tile_codes(t.m_tile) + (size_t)c * kLinearTileBytes, kLinearTileBytes);
+      }
+      chain_wait();
       Pos q;
-      bool ahead_of_it = true;
       for (int w = team; w < total && ok; w += teams) {
         const Tile t = tile_of<kCtas>(a.p, w, rank, split);
-        // a pair's second tile may lie past the last: it multiplies the last tile and stores nothing
-        const uint8_t* src = a.l.wq + (size_t)min(t.m_tile, a.l.padded_rows / kTileM - 1) * a.p.units * kLinearTileBytes;
+        const uint8_t* src = tile_codes(t.m_tile);
         for (int c = t.c0; c < t.c1; ++c, q.next(kCodes)) {
-          if (ahead_of_it && q.phase) {   // the ring is full: the bounded waits begin
-            chain_wait();
-            ahead_of_it = false;
-          }
           if (!ptx::mbar_wait_sleep(&ctl.code_empty[q.slot], q.phase ^ 1)) {
             ok = false;
             break;

@@ -88,9 +88,7 @@ def prepare_linear(weight: LinearWeights, gated: bool = False) -> dict:
     """Repack an NVFP4 matrix [N, K] for linear_w4 (once, untimed): any N, K a multiple of 16.
     gated: rows [0, N/2) are gate rows and the rest the matching up rows (a w13).
 
-    The state's tensors may be copied and rewritten in place like any others, but not by a kernel
-    that lets its successor start early (programmatic dependent launch; torch's own do not):
-    linear_w4 begins to read the weight ahead of the end of such a kernel."""
+    The state's tensors may be copied and rewritten in place like any others."""
     w, sf, gs = weight["w"], weight["w_sf"], weight["w_gs"]
     _require_cuda(w, "w")
     if w.dtype != torch.uint8 or w.dim() != 2 or 0 in w.shape:
