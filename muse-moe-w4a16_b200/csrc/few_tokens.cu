@@ -262,7 +262,7 @@ few_tokens(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
   __syncwarp();
   chain_wait();   // add is read and the outputs are written below
   __syncthreads();
-  const float scale = kW4 ? __ldg(a.gs) * kUnscale<kHalf> : 1.f;
+  const float scale = kW4 ? load_scale<kHalf>(a.gs) : 1.f;
   if (ranks > 1) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     const uint32_t mine = ptx::smem_u32(recv) + rank * toks * width * 4;

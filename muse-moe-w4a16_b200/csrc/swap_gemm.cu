@@ -259,7 +259,7 @@ swap_gemm(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUt
   };
   auto tile_epilogue = [&](const Tile& t, int buf) {
     const uint32_t acc = tmem + ((uint32_t)quarter << 21) + buf * a.p.bn;
-    const float gs = kW4 ? __ldg(a.l.gs) * kUnscale<kHalf> : 1.f;
+    const float gs = kW4 ? load_scale<kHalf>(a.l.gs) : 1.f;
     uint8_t* patch = patches + epi * kPatch;
     const int o0 = kGated ? t.m_tile * 64 + quarter * 16 : t.m_tile * kTileM + quarter * 32;
     const int outs = min(kOut, a.l.n_out - o0);

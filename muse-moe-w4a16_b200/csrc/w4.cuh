@@ -80,7 +80,10 @@ __device__ __forceinline__ void dequant_word(uint32_t w, uint32_t scale, uint32_
   }
 }
 template <bool kHalf> constexpr float kUnscale = kHalf ? 1.f : 256.f;
-
+// The global scale, from L2: this kernel may have started before the one that writes it ended, which a
+// load through the read-only path does not allow for.
+template <bool kHalf>
+__device__ __forceinline__ float load_scale(const float* gs) { return __ldcg(gs) * kUnscale<kHalf>; }
 
 __device__ __forceinline__ uint16_t round16(int dtype, float v) { return (uint16_t)(pack16(dtype, v, v) & 0xFFFF); }
 // (from L2: an addend may be the output that the kernel before wrote in place)

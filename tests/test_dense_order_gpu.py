@@ -60,3 +60,26 @@ def test_prepare_and_call_at_once(pkg, T):
     torch.cuda.synchronize()
     for i, got in enumerate(outs):
         assert torch.equal(got, want[i % 2]), i
+
+
+@pytest.mark.parametrize("T", [1, 12, 70, 400])
+def test_scale_rewritten_in_place(pkg, T):
+    """The global scale changes between calls, with nothing between the launches."""
+    state = pkg.prepare_linear(ref.random_w4(384, 1024, 7, DEV))
+    x = torch.randn((T, 1024), generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).to(DEV)
+    first = state["w_gs"].clone()
+    scales = [first, first * 4]
+    want = []
+    for s in scales:
+        torch.cuda.synchronize()
+        want.append(pkg.linear_w4(x, dict(state, w_gs=s)))
+    # a factor of four is exact, in fp32 and in bf16
+    assert torch.equal(want[1], want[0] * 4)
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(40):
+        torch.mul(first, 4.0 if i % 2 else 1.0, out=state["w_gs"])
+        outs += [pkg.linear_w4(x, state), pkg.linear_w4(x, state)]
+    torch.cuda.synchronize()
+    for i, got in enumerate(outs):
+        assert torch.equal(got, want[i // 2 % 2]), i
