@@ -14,6 +14,7 @@ import functools
 from typing import TypedDict
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -57,6 +58,14 @@ def _same(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) 
         raise _bad(f"{name} is on {t.device}, x on {device}")
     if t.dtype != dtype:
         raise _bad(f"{name} is {t.dtype}, x {dtype}")
+
+
+def _refuse_tangents(name: str, *tensors: torch.Tensor | None) -> None:
+    """A forward-mode tangent would be lost without an error: the kernels see the values alone."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level is open
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _bad(f"{name} has no forward-mode derivative: give it tensors without a tangent")
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -121,7 +130,8 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
     """x [..., K] times a prepared NVFP4 matrix: [..., N], or silu(gate) * up [..., N/2] for a gated
     one, plus `add` (same shape) if given. x is bf16 or fp16, and so are add and the result; any
     number of rows. Sums in fp32, one rounding. `out` receives the result if given; it may be `add`
-    itself. Inference only: it has no gradient."""
+    itself. Inference only: it has no gradient, and refuses tensors that want one or carry a
+    forward-mode tangent."""
     _require_cuda(x, "x")
     K, n_out, w, dev = state["cols"], state["n_out"], state["w"], x.device
     dtype = _DTYPES.get(x.dtype)
@@ -135,6 +145,7 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
         raise _bad(f"the weight is on {w.device} and its scale on {gs.device}, x on {dev}")
     if torch.is_grad_enabled() and (x.requires_grad or (add is not None and add.requires_grad)):
         raise _bad("linear_w4 has no gradient: call it under torch.no_grad()")
+    _refuse_tangents("linear_w4", x, gs, add, out)
     x2, ldx = _rows(x, K)
     T = x2.shape[0]
     if T > _MAX_ROWS:
@@ -238,7 +249,7 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, add: torch.T
     x [..., H], w13 [2I, H] (gate rows, then up rows, as the routed experts' w13), w2 [H, I], add of
     x's shape; all bf16 or all fp16; H and I multiples of 8. Sums in fp32; the inner activation and the
     gradients of the pre-activations are rounded to the tensors' type (fp16 ones overflow past
-    65504). Differentiable once in every tensor; a pass that needs gradients keeps the
+    65504). Differentiable once in every tensor, in reverse mode (a forward-mode tangent is refused); a pass that needs gradients keeps the
     pre-activations in fp32 (8 T I bytes). Equal inputs give equal bits, with or without gradients."""
     _require_cuda(x, "x")
     dev = x.device
@@ -259,6 +270,7 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, add: torch.T
         _same(add, "add", dev, x.dtype)
         if add.shape != x.shape:
             raise _bad(f"add must be {tuple(x.shape)}, got {tuple(add.shape)}")
+    _refuse_tangents("gated_ffn", x, w13, w2, add)
     if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad
                                     or (add is not None and add.requires_grad)):
         return _GatedFfn.apply(x, w13, w2, add)
