@@ -143,7 +143,7 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
     gs = state["w_gs"]
     if w.device != dev or gs.device != dev:
         raise _bad(f"the weight is on {w.device} and its scale on {gs.device}, x on {dev}")
-    if torch.is_grad_enabled() and (x.requires_grad or (add is not None and add.requires_grad)):
+    if torch.is_grad_enabled() and (x.requires_grad or gs.requires_grad or (add is not None and add.requires_grad)):
         raise _bad("linear_w4 has no gradient: call it under torch.no_grad()")
     _refuse_tangents("linear_w4", x, gs, add, out)
     x2, ldx = _rows(x, K)

@@ -45,6 +45,32 @@ def test_linear_refuses_tangents(pkg, monkeypatch, which, grad):
             linear_arguments("cpu"), which, grad)
 
 
+@pytest.mark.parametrize("which", ["x", "gs", "add", "out"])
+def test_linear_refuses_gradients(pkg, monkeypatch, which):
+    """Every floating-point tensor of a call, the global scale among them."""
+    from muse_moe_w4a16_b200 import dense
+    monkeypatch.setattr(dense, "_require_cuda", lambda t, name: None)
+    a = linear_arguments("cpu")
+    a[which] = a[which].requires_grad_()
+    state = {"cols": 64, "rows": 32, "n_out": 32, "gated": False, "w": torch.zeros(1024, dtype=torch.uint8), "w_gs": a["gs"]}
+    with pytest.raises(pkg.MuseError, match="gradient") as e:
+        pkg.linear_w4(a["x"], state, add=a["add"], out=a["out"])
+    assert e.value.code == -1
+
+
+@gpu
+def test_linear_with_a_trained_scale(pkg):
+    """A scale that wants a gradient: refused while gradients are on, served without."""
+    weight = ref.random_w4(32, 64, 1, DEV)
+    x = torch.ones((2, 64), dtype=torch.bfloat16, device=DEV)
+    want = pkg.linear_w4(x, pkg.prepare_linear(weight))
+    state = pkg.prepare_linear(dict(weight, w_gs=weight["w_gs"].clone().requires_grad_()))
+    with pytest.raises(pkg.MuseError):
+        pkg.linear_w4(x, state)
+    with torch.no_grad():
+        assert torch.equal(pkg.linear_w4(x, state), want)
+
+
 @pytest.mark.parametrize("grad", [True, False])
 @pytest.mark.parametrize("which", ["x", "w13", "w2", "add"])
 def test_ffn_refuses_tangents(pkg, monkeypatch, which, grad):
