@@ -373,9 +373,9 @@ int muse_moe_forward_noalloc(const void* x, const int32_t* topk_ids, const float
  *
  * muse_moe_linear_prepared_size / muse_moe_prepare_linear: a row-major NVFP4 matrix w u8 [rows,
  * cols/2], w_sf e4m3 [rows, cols/16] in the experts' tile order, each tile's scales behind its codes
- * (any rows; cols a multiple of 16; rows and columns padded to 128 with zero codes). gated: rows [0, rows/2) are gate rows, the
- * rest the matching up rows. No counterpart in the reference, whose prepare (baseline.py:82-103)
- * repacks routed experts only.
+ * (rows and cols up to 2^24, cols a multiple of 16, both padded to 128 with zero codes; fewer than 2^31
+ * tiles). gated: rows [0, rows/2) are gate rows, the rest the matching up rows. No counterpart in
+ * the reference, whose prepare (baseline.py:82-103) repacks routed experts only.
  */
 int muse_moe_linear_prepared_size(int rows, int cols, int gated, size_t* bytes);
 int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int cols, int gated, uint8_t* out,

@@ -139,7 +139,7 @@ extern "C" const char* muse_moe_error_string(int code) {
     case MUSE_ERR_INVALID_ARGUMENT: return "invalid argument (null pointer or bad size)";
     case MUSE_ERR_UNSUPPORTED_SHAPE:
       return "unsupported shape (layer calls: hidden and inter must be multiples of 128, top_k <= 16, "
-             "local_count <= 256; linear_w4: cols of 16; ffn: hidden and inter of 8)";
+             "local_count <= 256; linear_w4: cols of 16, rows and cols up to 2^24; ffn: hidden and inter of 8)";
     case MUSE_ERR_WORKSPACE_TOO_SMALL: return "workspace smaller than muse_moe_workspace_size() (ffn calls: muse_moe_ffn_workspace_size())";
     case MUSE_ERR_NO_DEVICE: return "no sm_100 CUDA device / driver entry point available";
     case MUSE_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait expired";

@@ -17,14 +17,13 @@ namespace {
 
 // ---------------------------------------------------------------------------- repack
 
-// One CTA per (128-row tile, 128-code chunk), thread = tile row. Rows and codes past the
+// One CTA per (128-row tile, 128-code chunk), chunks innermost, thread = tile row. Rows and codes past the
 // matrix are zero codes with zero scales. gate_up > 0: rows of gate and up interleave by 16 as
 // in a w13 tile; `gate_up` is I, padded to 64 rows per half on its own.
 __global__ void __launch_bounds__(kTileM)
 prepare_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int cols,
-                      int gate_up, uint8_t* __restrict__ out) {
-  const int kc = blockIdx.x, m = blockIdx.y, r = threadIdx.x;
-  const int k_chunks = gridDim.x;
+                      int gate_up, int k_chunks, uint8_t* __restrict__ out) {
+  const int m = blockIdx.x / k_chunks, kc = blockIdx.x % k_chunks, r = threadIdx.x;
   int src = m * kTileM + r;
   bool row_ok = src < rows;
   if (gate_up > 0) {
@@ -32,7 +31,7 @@ prepare_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
     row_ok = j < gate_up;
     src = (r & 16) ? gate_up + j : j;
   }
-  const size_t tile = (size_t)m * k_chunks + kc;
+  const size_t tile = blockIdx.x;
   uint8_t* dst = out + tile * kLinearTileBytes + r * kRowCodeBytes;
   uint8_t* sdst = out + tile * kLinearTileBytes + kTileCodeBytes + r * kRowScaleBytes;
   const uint8_t* c = codes + (size_t)src * (cols / 2) + (size_t)kc * kRowCodeBytes;
@@ -50,13 +49,17 @@ prepare_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
 }
 
 int padded(int v, int to) { return (v + to - 1) / to * to; }
+int padded_rows_of(int rows, int gated) { return gated ? 2 * padded(rows / 2, 64) : padded(rows, kTileM); }
+long long tiles_of(int rows, int cols, int gated) {
+  return (long long)(padded_rows_of(rows, gated) / kTileM) * (padded(cols, kChunkK) / kChunkK);
+}
 
 int check_linear(int rows, int cols, int gated) {
   if (rows <= 0 || cols <= 0 || (gated != 0 && gated != 1) || (gated && rows % 2)) return MUSE_ERR_INVALID_ARGUMENT;
   if (cols % kBlock || rows > (1 << 24) || cols > (1 << 24)) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  if (tiles_of(rows, cols, gated) > 0x7FFFFFFF) return MUSE_ERR_UNSUPPORTED_SHAPE;   // a grid's x
   return MUSE_OK;
 }
-int padded_rows_of(int rows, int gated) { return gated ? 2 * padded(rows / 2, 64) : padded(rows, kTileM); }
 
 bool misaligned(const void* p, unsigned to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
@@ -69,7 +72,7 @@ extern "C" int muse_moe_linear_prepared_size(int rows, int cols, int gated, size
   if (!bytes) return MUSE_ERR_INVALID_ARGUMENT;
   const int rc = check_linear(rows, cols, gated);
   if (rc) return rc;
-  *bytes = (size_t)(padded_rows_of(rows, gated) / kTileM) * (padded(cols, kChunkK) / kChunkK) * kLinearTileBytes;
+  *bytes = (size_t)tiles_of(rows, cols, gated) * kLinearTileBytes;
   return MUSE_OK;
 }
 
@@ -78,9 +81,8 @@ extern "C" int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, in
   const int rc = check_linear(rows, cols, gated);
   if (rc) return rc;
   if (!w || !w_sf || !out || misaligned(w, 8) || misaligned(out, 16)) return MUSE_ERR_INVALID_ARGUMENT;
-  const dim3 grid(padded(cols, kChunkK) / kChunkK, padded_rows_of(rows, gated) / kTileM);
-  if (grid.y > 65535) return MUSE_ERR_UNSUPPORTED_SHAPE;
-  prepare_linear_kernel<<<grid, kTileM, 0, (cudaStream_t)stream>>>(w, w_sf, rows, cols, gated ? rows / 2 : 0, out);
+  prepare_linear_kernel<<<(unsigned)tiles_of(rows, cols, gated), kTileM, 0, (cudaStream_t)stream>>>(
+      w, w_sf, rows, cols, gated ? rows / 2 : 0, padded(cols, kChunkK) / kChunkK, out);
   return last_launch_status();
 }
 
