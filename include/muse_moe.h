@@ -384,8 +384,8 @@ int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int
 /*
  * out[t, n] = gs * sum_k x[t, k] * e2m1[n, k] * e4m3[n, k/16] (+ add[t, n]), or with gated
  * out[t, i] = silu(gate) * up (+ add), [tokens, rows/2]. rows, cols, gated as at the prepare call.
- * x: 16-byte aligned, ldx a multiple of 8. fp32 sums over weights that are exact in 16 bits, one
- * rounding at the end. No counterpart in the reference.
+ * x and wp: 16-byte aligned, ldx a multiple of 8; w_gs, add and out: aligned to their type. fp32
+ * sums over weights that are exact in 16 bits, one rounding at the end. No counterpart in the reference.
  */
 int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int rows, int cols, int gated,
                        const uint8_t* wp, const float* w_gs, const void* add, long long ld_add, void* out, long long ldo, muse_stream_t stream);

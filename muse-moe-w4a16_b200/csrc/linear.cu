@@ -96,6 +96,7 @@ extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int t
   if (tokens == 0) return MUSE_OK;
   if (tokens > (1 << 28)) return MUSE_ERR_UNSUPPORTED_SHAPE;
   if (!x || !wp || !w_gs || !out || misaligned(x, 16) || ldx % 8 || misaligned(wp, 16) ||
+      misaligned(w_gs, 4) || misaligned(add, 2) || misaligned(out, 2) ||
       (tokens > 1 && (ldx < cols || ldo < n_out || (add && ld_add < n_out))))
     return MUSE_ERR_INVALID_ARGUMENT;
   LinearArgs a{};
