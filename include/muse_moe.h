@@ -391,6 +391,18 @@ int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int tokens, int 
                        const uint8_t* wp, const float* w_gs, const void* add, long long ld_add, void* out, long long ldo, muse_stream_t stream);
 
 /*
+ * How a dense product would run, from the same rules the launches use: a diagnostic for tests.
+ *   plan[0] 0: few tokens; 1: weight rows on the MMA's M side; 2: tokens on the M side;
+ *   plan[1] tile width (tokens for 1, columns for 2), plan[2] output tiles, plan[3] tiles whose K is
+ *           not split, plan[4] parts of K of the others (1: none is split), plan[5] output tiles of
+ *           the busiest group of CTAs (more than one: accumulators alternate).
+ * For few tokens the rest is 0. plan has room for 6 ints. linear_plan: linear_w4's product. ffn_plan:
+ * product 0 x . W13^T, 1 h . W2^T, 2 dy . W2, 3 [da db] . W13, 4 [da db]^T x, 5 dy^T h; tokens > 0.
+ */
+int muse_moe_linear_plan(int tokens, int rows, int cols, int gated, int* plan);
+int muse_moe_ffn_plan(int product, int tokens, int hidden, int inter, int* plan);
+
+/*
  * The gated feed-forward block with 16-bit weights w13 [2 * inter, hidden] (gate rows, then up
  * rows) and w2 [hidden, inter]: out = (silu(x . Wg^T) * (x . Wu^T)) . W2^T (+ add), [tokens, hidden].
  * ab: null, or fp32 [tokens, 2 * inter] that receives the pre-activations for the backward call.

@@ -63,6 +63,8 @@ SIGNATURES: dict[str, tuple] = {
     "muse_moe_linear_prepared_size": (_I, [_I, _I, _I, _SIZE_P]),
     "muse_moe_prepare_linear": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "muse_moe_linear_w4": (_I, [_P, _L, _I, _I, _I, _I, _I, _P, _P, _P, _L, _P, _L, _P]),
+    "muse_moe_linear_plan": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I)]),
+    "muse_moe_ffn_plan": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I)]),
     "muse_moe_ffn_workspace_size": (_I, [_I, _I, _I, _I, _SIZE_P]),
     "muse_moe_ffn_forward": (_I, [_P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _P, _P, ctypes.c_size_t, _P]),
     "muse_moe_ffn_backward": (_I, [_P, _L, _P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _P, _P,
@@ -147,6 +149,17 @@ def workspace_size(tokens: int, top_k: int, local_count: int, hidden: int, inter
     n = ctypes.c_size_t(0)
     call("muse_moe_workspace_size", tokens, top_k, local_count, hidden, inter, ctypes.byref(n))
     return int(n.value)
+
+
+def dense_plan(product: str, tokens: int, *sizes: int) -> dict:
+    """How a dense product would run (include/muse_moe.h): "linear" or "gated" with sizes rows, cols,
+    else one of "gate", "down", "dgate", "dx", "dw13", "dw2" with sizes hidden, inter."""
+    arr = (ctypes.c_int * 6)()
+    if product in ("linear", "gated"):
+        call("muse_moe_linear_plan", tokens, *sizes, int(product == "gated"), arr)
+    else:
+        call("muse_moe_ffn_plan", ("gate", "down", "dgate", "dx", "dw13", "dw2").index(product), tokens, *sizes, arr)
+    return dict(zip(("kernel", "tile", "tiles", "whole", "splits", "per_group"), arr))
 
 
 def launch_plan(tokens: int, top_k: int, local_count: int, hidden: int, inter: int,

@@ -11,6 +11,8 @@
 
 namespace muse {
 
+constexpr int kMaxRows = 1 << 28;   // tokens of one call
+
 // Element type of a dense operator's tensors (the ABI's `dtype`).
 enum DenseType : int { kBf16 = 0, kFp16 = 1 };
 
@@ -58,6 +60,19 @@ int make_operand_map(CUtensorMap* map, const DenseOperand& o, int extent, int k,
 // Map of gated weights [gate rows; up rows] (K-major) as [inter / 8][2][8] rows: a box is 64 k x eight
 // gate and the eight matching up rows x eight such groups, 128 rows in that order.
 int make_gated_map(CUtensorMap* map, const DenseOperand& o, int inter, int k, int dtype);
+
+// How a product runs (muse_moe_linear_plan, muse_moe_ffn_plan), in the order of their plan's entries.
+struct PlanInfo {
+  long long kernel, tile, tiles, whole, splits, per_group;
+};
+inline int put_plan(const PlanInfo& p, int* out) {
+  if (p.tiles > (1 << 30)) return MUSE_ERR_UNSUPPORTED_SHAPE;   // more than any launch takes
+  const long long v[6] = {p.kernel, p.tile, p.tiles, p.whole, p.splits, p.per_group};
+  for (int i = 0; i < 6; ++i) out[i] = (int)v[i];
+  return MUSE_OK;
+}
+PlanInfo dense_plan(int m, int n, int k, int mode, bool b_k_major);
+PlanInfo swap_dense_plan(int m, int n, int k);
 
 // The forward products (modes kStore and kGate, both operands along k) with the weights on the MMA's
 // M side (swap_gemm.cu), and both forms' estimated times in SM clocks.

@@ -471,7 +471,7 @@ constexpr int kPairs = 74;  // 148 SMs, two to a pair
 
 struct Plan {
   int bn, tiles_m, tiles_n, kb_total, whole, splits, kb_per_split;
-  int tail() const { return splits > 1 ? tiles_m * tiles_n - whole : 0; }
+  int tail() const { return splits > 1 ? (int)((long long)tiles_m * tiles_n - whole) : 0; }
 };
 
 // Tile width, and the split of K for the tail: the tiles that do not fill a wave of all pairs are cut
@@ -581,6 +581,12 @@ double dense_cost(int m, int n, int k, int mode, bool b_k_major) {
   double cost;
   make_plan(m, n, k, mode, b_k_major, &cost);
   return cost;
+}
+
+PlanInfo dense_plan(int m, int n, int k, int mode, bool b_k_major) {
+  const Plan p = make_plan(m, n, k, mode, b_k_major);
+  const long long tiles = (long long)p.tiles_m * p.tiles_n, items = p.whole + (long long)p.tail() * p.splits;
+  return {2, p.bn, tiles, tiles - p.tail(), p.splits, (items + kPairs - 1) / kPairs};
 }
 
 size_t dense_scratch_bytes(int m, int n, int k, int mode, bool b_k_major) {

@@ -18,7 +18,7 @@ constexpr size_t kAlign = 256;
 
 int check_ffn(int tokens, int hidden, int inter) {
   if (tokens < 0 || hidden <= 0 || inter <= 0) return MUSE_ERR_INVALID_ARGUMENT;
-  if (hidden % 8 || inter % 8 || hidden > (1 << 24) || inter > (1 << 24) || tokens > (1 << 28))
+  if (hidden % 8 || inter % 8 || hidden > (1 << 24) || inter > (1 << 24) || tokens > kMaxRows)
     return MUSE_ERR_UNSUPPORTED_SHAPE;
   return MUSE_OK;
 }
@@ -34,6 +34,12 @@ int (*forward_product(int t, int n, int k, int mode))(const DenseGemm&, cudaStre
 size_t forward_scratch(int t, int n, int k, int mode) {
   if (forward_product(t, n, k, mode) != launch_dense_gemm) return 0;
   return dense_scratch_bytes(t, n, k, mode, true);
+}
+
+PlanInfo forward_plan(int t, int n, int k, int mode) {
+  const auto product = forward_product(t, n, k, mode);
+  if (product == launch_few_dense) return {};
+  return product == launch_swap_dense ? swap_dense_plan(t, n, k) : dense_plan(t, n, k, mode, true);
 }
 
 size_t up(size_t v) { return align_up(v, kAlign); }
@@ -75,6 +81,21 @@ extern "C" int muse_moe_ffn_workspace_size(int tokens, int hidden, int inter, in
   if (rc) return rc;
   *bytes = tokens == 0 ? 0 : ffn_layout(tokens, hidden, inter, backward != 0).total;
   return MUSE_OK;
+}
+
+extern "C" int muse_moe_ffn_plan(int product, int tokens, int hidden, int inter, int* plan) {
+  const int rc = check_ffn(tokens, hidden, inter);
+  if (rc) return rc;
+  if (!plan || tokens == 0) return MUSE_ERR_INVALID_ARGUMENT;
+  switch (product) {
+    case 0: return put_plan(forward_plan(tokens, 2 * inter, hidden, kGate), plan);
+    case 1: return put_plan(forward_plan(tokens, hidden, inter, kStore), plan);
+    case 2: return put_plan(dense_plan(tokens, inter, hidden, kDGate, false), plan);
+    case 3: return put_plan(dense_plan(tokens, hidden, 2 * inter, kStore, false), plan);
+    case 4: return put_plan(dense_plan(2 * inter, hidden, tokens, kStore, false), plan);
+    case 5: return put_plan(dense_plan(hidden, inter, tokens, kStore, false), plan);
+    default: return MUSE_ERR_INVALID_ARGUMENT;
+  }
 }
 
 extern "C" int muse_moe_ffn_forward(const void* x, long long ldx, int dtype, int tokens, int hidden, int inter,

@@ -76,6 +76,17 @@ extern "C" int muse_moe_linear_prepared_size(int rows, int cols, int gated, size
   return MUSE_OK;
 }
 
+extern "C" int muse_moe_linear_plan(int tokens, int rows, int cols, int gated, int* plan) {
+  const int rc = check_linear(rows, cols, gated);
+  if (rc) return rc;
+  if (!plan || tokens <= 0) return MUSE_ERR_INVALID_ARGUMENT;
+  if (tokens > kMaxRows) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  return put_plan(streams_w4(tokens, rows, cols)
+                      ? PlanInfo{}
+                      : linear_gemm_plan(tokens, padded_rows_of(rows, gated), padded(cols, kChunkK) / kChunkK),
+                  plan);
+}
+
 extern "C" int muse_moe_prepare_linear(const uint8_t* w, const uint8_t* w_sf, int rows, int cols, int gated,
                                        uint8_t* out, muse_stream_t stream) {
   const int rc = check_linear(rows, cols, gated);
@@ -94,7 +105,7 @@ extern "C" int muse_moe_linear_w4(const void* x, long long ldx, int dtype, int t
   const int n_out = gated ? rows / 2 : rows;
   if (tokens < 0 || (dtype != kBf16 && dtype != kFp16)) return MUSE_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return MUSE_OK;
-  if (tokens > (1 << 28)) return MUSE_ERR_UNSUPPORTED_SHAPE;
+  if (tokens > kMaxRows) return MUSE_ERR_UNSUPPORTED_SHAPE;
   if (!x || !wp || !w_gs || !out || misaligned(x, 16) || ldx % 8 || misaligned(wp, 16) ||
       misaligned(w_gs, 4) || misaligned(add, 2) || misaligned(out, 2) ||
       (tokens > 1 && (ldx < cols || ldo < n_out || (add && ld_add < n_out))))

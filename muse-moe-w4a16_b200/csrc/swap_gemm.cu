@@ -662,12 +662,25 @@ int launch_any(const LinearArgs& l, const GemmPlan& p, const CUtensorMap& mw, in
   return p.ctas == 2 ? launch_typed<2, kW4>(mx, mw, a, dtype, gated, st) : launch_typed<1, kW4>(mx, mw, a, dtype, gated, st);
 }
 
+PlanInfo info(const GemmPlan& p) {
+  const long long tiles = (long long)p.tiles_m * p.tiles_n, groups = kSms / p.ctas;
+  return {1, p.bn, tiles, p.splits > 1 ? 0 : tiles, p.splits, p.splits > 1 ? 1 : (tiles + groups - 1) / groups};
+}
+
 int padded_rows_of(const DenseGemm& g) { return (g.n + kTileM - 1) / kTileM * kTileM; }
 
 }  // namespace
 
 int launch_linear_gemm(const LinearArgs& l, int dtype, bool gated, int* error_flag, cudaStream_t st) {
   return launch_any<true>(l, make_plan<true>(l.tokens, l.padded_rows, l.k_chunks), CUtensorMap{}, dtype, gated, error_flag, st);
+}
+
+PlanInfo linear_gemm_plan(int tokens, int padded_rows, int k_chunks) {
+  return info(make_plan<true>(tokens, padded_rows, k_chunks));
+}
+
+PlanInfo swap_dense_plan(int m, int n, int k) {
+  return info(make_plan<false>(m, (n + kTileM - 1) / kTileM * kTileM, (k + 63) / 64));
 }
 
 double swap_dense_cost(int m, int n, int k) {

@@ -27,8 +27,9 @@ struct LinearArgs {
   uint32_t m16, m64;         // 16 and 64 (see dequant_word)
 };
 
-// The product for more than a few tokens.
+// The product for more than a few tokens, and how it runs.
 int launch_linear_gemm(const LinearArgs& a, int dtype, bool gated, int* error_flag, cudaStream_t st);
+PlanInfo linear_gemm_plan(int tokens, int padded_rows, int k_chunks);
 
 __device__ __forceinline__ uint32_t mul2_bf16(uint32_t a, uint32_t b) {
   uint32_t d;
