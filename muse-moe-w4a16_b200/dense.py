@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import types
 from typing import TypedDict
 
 import torch
@@ -60,10 +61,12 @@ def _same(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) 
         raise _bad(f"{name} is {t.dtype}, x {dtype}")
 
 
+# Where no dual level is open (_current_level < 0) no tensor has a tangent, and a call need not look.
+_duals = forward_ad if hasattr(forward_ad, "_current_level") else types.SimpleNamespace(_current_level=0)
+
+
 def _refuse_tangents(name: str, *tensors: torch.Tensor | None) -> None:
     """A forward-mode tangent would be lost without an error: the kernels see the values alone."""
-    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level is open
-        return
     if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise _bad(f"{name} has no forward-mode derivative: give it tensors without a tangent")
 
@@ -145,7 +148,8 @@ def linear_w4(x: torch.Tensor, state: dict, add: torch.Tensor | None = None,
         raise _bad(f"the weight is on {w.device} and its scale on {gs.device}, x on {dev}")
     if torch.is_grad_enabled() and (x.requires_grad or gs.requires_grad or (add is not None and add.requires_grad)):
         raise _bad("linear_w4 has no gradient: call it under torch.no_grad()")
-    _refuse_tangents("linear_w4", x, gs, add, out)
+    if _duals._current_level >= 0:
+        _refuse_tangents("linear_w4", x, gs, add, out)
     x2, ldx = _rows(x, K)
     T = x2.shape[0]
     if T > _MAX_ROWS:
@@ -270,7 +274,8 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, add: torch.T
         _same(add, "add", dev, x.dtype)
         if add.shape != x.shape:
             raise _bad(f"add must be {tuple(x.shape)}, got {tuple(add.shape)}")
-    _refuse_tangents("gated_ffn", x, w13, w2, add)
+    if _duals._current_level >= 0:
+        _refuse_tangents("gated_ffn", x, w13, w2, add)
     if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad
                                     or (add is not None and add.requires_grad)):
         return _GatedFfn.apply(x, w13, w2, add)
