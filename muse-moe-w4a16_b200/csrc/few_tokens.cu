@@ -10,10 +10,12 @@
 // is the lanes' -- so nothing is shuffled. A CTA pushes its sums to the ranks that own the outputs
 // (16-byte stores to distributed shared memory, one cluster barrier), which add them in rank order.
 // Sixteen warps with half of a stage each measured slower (13.0 against 8.7 us at 1 x 7168 x 4096
-// gated): for NVFP4 the instructions per code are what keeps the stream from HBM's rate.
-// Bound by the weights' bytes (the block of 1 x 7168 x 2048 in 16 bits: 20.0 us, 4.4 TB/s over both
-// products; NVFP4 1 x 7168 x 4096 gated: 8.8 us, 1.9 TB/s); the smallest sizes by launch, first-byte
-// and cluster latency (1 x 1024 x 1024: 3.2 us).
+// gated).
+// 16 bits are bound by the weights' bytes (the block of 1 x 7168 x 2048: 20.1 us, 4.4 TB/s over both
+// products). NVFP4 is bound by latency: 1 x 7168 x 4096 gated takes 9.0 us, 1.8 TB/s, with a CTA's seven
+// stages in flight from the start; its warps issue in 37 % of the cycles they are resident, the logic
+// pipe is 33 % busy, and they wait at the barriers, for the first bytes and for one another's sums. So do
+// the smallest sizes (1 x 1024 x 1024: 3.3 us).
 #undef MUSE_TRACE  // these kernels record no stamps
 #include "few_tokens.cuh"
 

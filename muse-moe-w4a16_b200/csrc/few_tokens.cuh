@@ -7,14 +7,26 @@ namespace muse {
 
 // The most tokens of these calls.
 constexpr int kFewTokens = 32;
-// A forward product of 16-bit weights [n, k] that is streamed: few tokens, or a weight so small that the
-// other kernel's second launch for its split K costs more than it gains (24 x 2048 x 768 block: 16.4
-// against 19.6 us a call; 32 x 7168 x 2048: 28.8 against 23.5).
+// A forward product of 16-bit weights [n, k] that is streamed: few tokens, or a small weight, where set-up
+// and exchange cost the tensor-core kernels more than the stream's mma.sync does. Device times of whole
+// blocks, both products streamed / both on the tensor cores, us:
+//   block           8 tokens     9            16           17           32
+//   2048 x 768      8.3 / 12.6   10.5 / 12.7  11.6 / 12.7  12.2 / 12.7  14.2 / 12.7
+//   4096 x 1024     10.5 / 14.3  13.4 / 14.3  14.2 / 14.2  15.9 / 14.3  17.8 / 14.3
+//   4096 x 2048     15.1 / 19.3  19.2 / 19.3  18.5 / 19.0  19.9 / 19.1  19.7 / 19.1
+//   7168 x 2048     19.6 / 24.3  22.3 / 24.3  22.4 / 24.4  25.6 / 24.4  27.1 / 24.5
+// From 9 to 16 tokens the stream is level or ahead at all of these, from 17 on behind at most: one limit
+// for both, which costs up to a quarter where it is farthest off (4096 x 1024 at 32 tokens).
 inline bool streams_dense(int tokens, int n, int k) {
   return tokens <= 8 || (tokens <= kFewTokens && (long long)n * k <= (8LL << 20));
 }
-// A product with an NVFP4 weight that is streamed: likewise (24 x 4096 x 4096: 10.4 against 11.7 us, 17 x
-// 7168 x 4096: 15.6 against 13.8).
+// A product with an NVFP4 weight that is streamed: likewise (streamed / tensor cores, us on the device):
+//   rows x columns  8 tokens    16           17           32
+//   2048 x 2048     4.1 / 8.5   6.0 / 8.5    6.3 / 8.5    7.0 / 8.6
+//   4096 x 4096     7.4 / 10.4  9.8 / 10.4   10.3 / 10.4  10.6 / 10.4
+//   5120 x 4096     8.8 / 12.7  11.6 / 12.7  14.3 / 12.7  15.8 / 12.8
+//   8192 x 7168     13.1 / 20.1 17.0 / 20.1  22.5 / 20.2  23.7 / 20.2
+// Above 16 tokens they cross between 16 and 20 M codes.
 inline bool streams_w4(int tokens, int rows, int cols) {
   return tokens <= 16 || (tokens <= kFewTokens && (long long)rows * cols <= (20LL << 20));
 }

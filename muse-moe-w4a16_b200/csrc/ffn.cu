@@ -7,7 +7,7 @@
 // Roundings to 16 bits besides the results': h (the second product's operand), da and db (the
 // operands of dx and dW13), each once from fp32. The pre-activations are kept in fp32 for the
 // backward pass, 8 T I bytes: kept in 16 bits their rounding would enter da, db and h a second
-// time. h is recomputed from them, to the same bits, rather than kept.
+// time. h is recomputed from them rather than kept.
 #include "few_tokens.cuh"
 #include "kernels.cuh"
 

@@ -22,9 +22,11 @@
 // CTAs. Each group owns every splits-th 32-token chunk of the tile's outputs and receives the others'
 // accumulators of it, as fragments, through distributed shared memory (the rings are done by then): the
 // owner adds them to its own, in split order, and finishes the chunk. One launch, no scratch memory.
-// Tens of tokens are bound by set-up, exchange and the dequantisation more than by weight bytes (64 x
-// 4096 x 8192 gated: 14.4 us, 1.4 TB/s), hundreds by the tensor pipe (1000 x 4096 x 4096: 32 us; 2000 x
-// 7168 x 4096 gated: 100 us, 1.17 PFLOP/s, in a loop under the power limit).
+// Tens of tokens are bound by set-up, exchange and the stages' hand-over more than by weight bytes (64 x
+// 4096 x 8192 gated: 14.5 us, 1.4 TB/s, tensor pipe 19 % active). With NVFP4 weights hundreds and
+// thousands are bound by a stage's dequantisation and hand-over, longer than its MMAs (4096 x 4096 x 4096:
+// tensor pipe 75 % active, issue slots 48 %; 106 us at full clock, 119 in a loop under the power limit;
+// 1000 x 4096 x 4096: 28 and 32 us; 2000 x 7168 x 4096 gated: 88 and 103 us).
 #undef MUSE_TRACE  // these kernels record no stamps
 #include "kernels.cuh"
 #include "pair.cuh"
